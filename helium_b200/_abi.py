@@ -48,6 +48,13 @@ class HeConv2dFusion(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("out_dtype", "has_bias", "bias_dtype", "has_resid", "has_gate", "want_stats")]
 
 
+class HeGroupNormParams(C.Structure):
+    """struct he_group_norm_params of include/helium_b200.h."""
+
+    _fields_ = [("batch", C.c_int32), ("channels", C.c_int32), ("positions", C.c_int64), ("groups", C.c_int32), ("dtype", C.c_int32),
+                ("activation", C.c_int32), ("eps", C.c_float)]
+
+
 #: every symbol include/helium_b200.h declares: name -> (restype, argtypes)
 SIGNATURES = {
     "he_ctx_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
@@ -62,6 +69,7 @@ SIGNATURES = {
     "he_plan_fused_matmul": (C.c_int32, [C.c_void_p, C.POINTER(HeGraphDesc), C.POINTER(C.c_void_p)]),
     "he_plan_conv2d": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(HeConv2dParams), C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                    C.POINTER(HeConv2dFusion), C.POINTER(C.c_void_p)]),
+    "he_plan_group_norm": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(HeGroupNormParams), C.POINTER(C.c_void_p)]),
     "he_bn_finalize": (C.c_int32, [C.c_void_p, C.c_int64] + [C.c_void_p] * 8 + [C.c_int32, C.c_void_p]),
     "he_bn_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "he_bn_apply": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,

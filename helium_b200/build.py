@@ -39,6 +39,7 @@ SOURCES = [
     "comm.cu",
     "conv.cu",
     "train_ops.cu",
+    "group_norm.cu",
 ]
 
 NVCC_FLAGS = [

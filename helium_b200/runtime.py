@@ -6,16 +6,18 @@ goes through `he_launch`; nothing here computes on the host.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import List, Optional, Sequence
 
 import numpy as np
 
 from . import ir
-from ._abi import HeConv2dFusion, HeConv2dParams
+from ._abi import HeConv2dFusion, HeConv2dParams, HeGroupNormParams
 from ._lib import HeliumError, check, lib
 
 _TORCH_DTYPES = None
+_NO_CONTEXT = contextlib.nullcontext()
 
 
 def _torch():
@@ -81,6 +83,8 @@ class Plan:
         self.n_inputs = n_inputs
         self.ctx = ctx
         self._workspace = None
+        self._in_specs = None       # (shape, dtype) of every input, for the plans whose launches are checked
+        self._ws_bytes = None
 
     # -- constructors ------------------------------------------------------------------------------
     @staticmethod
@@ -145,6 +149,26 @@ class Plan:
             dtypes.append(ir.F32)
         return Plan(h, shapes, dtypes, n_in, ctx)
 
+    @staticmethod
+    def group_norm(ctx: Optional[Context], direction: str, batch: int, positions: int, channels: int, groups: int, dtype: int = ir.BF16,
+                   activation: str = "none", eps: float = 1e-5) -> "Plan":
+        """he_plan_group_norm over [batch, positions, channels] (NHWC, H and W flattened).  direction: "fwd" (inputs x,
+        gamma, beta; outputs y, mean, rstd) or "bwd" (inputs dy, x, gamma, beta, mean, rstd; outputs dx, dgamma, dbeta).
+        activation: "none", "relu", "silu" or "gelu"."""
+        d = {"fwd": 0, "bwd": 1}[direction]
+        prm = HeGroupNormParams(batch, channels, positions, groups, dtype, {"none": 0, "relu": 1, "silu": 2, "gelu": 3}[activation], eps)
+        h = C.c_void_p()
+        check(lib.he_plan_group_norm(ctx._h if ctx else None, d, C.byref(prm), C.byref(h)))
+        x = (batch, positions, channels)
+        if d == 0:
+            plan = Plan(h, [x, (batch, groups), (batch, groups)], [dtype, ir.F32, ir.F32], 3, ctx)
+            plan._in_specs = [(x, dtype), ((channels,), ir.F32), ((channels,), ir.F32)]
+        else:
+            plan = Plan(h, [x, (channels,), (channels,)], [dtype, ir.F32, ir.F32], 6, ctx)
+            plan._in_specs = [(x, dtype), (x, dtype), ((channels,), ir.F32), ((channels,), ir.F32), ((batch, groups), ir.F32),
+                              ((batch, groups), ir.F32)]
+        return plan
+
     # -- queries -----------------------------------------------------------------------------------
     @property
     def workspace_bytes(self) -> int:
@@ -191,6 +215,8 @@ class Plan:
         for t in inputs:
             if not t.is_cuda or not t.is_contiguous():
                 raise ValueError("inputs must be contiguous CUDA tensors")
+        if self._in_specs is not None:
+            return self._launch_checked(torch, inputs, outputs, stream)
         if outputs is None:
             outputs = self.alloc_outputs(inputs[0].device if inputs else "cuda")
         ws = self.workspace_bytes
@@ -200,6 +226,47 @@ class Plan:
         if ws:
             wptr = (self._workspace.data_ptr() + 255) // 256 * 256
         self.launch_ptrs([t.data_ptr() for t in inputs], [t.data_ptr() for t in outputs], wptr, stream)
+        return outputs
+
+    def _launch_checked(self, torch, inputs, outputs, stream):
+        """`launch` of the plans that know their operands' shapes: every tensor is checked, the stream is the current one
+        of the plan's device, and the workspace belongs to this launch alone (taken from torch's allocator on the launching
+        stream: part of the graph's pool under capture), so launches on several streams and several captured graphs never
+        share one."""
+        dev = self.ctx.device if self.ctx else None
+
+        def checked(t, spec, what, i):
+            if tuple(t.shape) != spec[0] or t.dtype != _TORCH_DTYPES[spec[1]]:
+                raise ValueError(f"{what} {i} must be {_TORCH_DTYPES[spec[1]]} {spec[0]}, got {t.dtype} {tuple(t.shape)}")
+            if dev is not None and t.device.index != dev:
+                raise ValueError(f"{what} {i} is on {t.device}, the plan on cuda:{dev}")
+            return t.data_ptr()
+
+        ins = [checked(t, spec, "input", i) for i, (t, spec) in enumerate(zip(inputs, self._in_specs))]
+        current = torch.cuda.current_stream(dev)
+        if stream is None:
+            target = current
+        else:
+            target = torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream
+        with torch.cuda.stream(target) if target != current else _NO_CONTEXT:
+            if outputs is None:
+                outputs = self.alloc_outputs(inputs[0].device)
+                outs = [t.data_ptr() for t in outputs]
+            else:
+                if len(outputs) != len(self.out_shapes):
+                    raise ValueError(f"plan writes {len(self.out_shapes)} outputs, got {len(outputs)}")
+                outs = []
+                for i, t in enumerate(outputs):
+                    if not t.is_cuda or not t.is_contiguous():
+                        raise ValueError("outputs must be contiguous CUDA tensors")
+                    outs.append(checked(t, (tuple(self.out_shapes[i]), self.out_dtypes[i]), "output", i))
+            if self._ws_bytes is None:
+                self._ws_bytes = self.workspace_bytes
+            wptr = 0
+            if self._ws_bytes:
+                ws = torch.empty(self._ws_bytes + 256, dtype=torch.uint8, device=inputs[0].device)
+                wptr = (ws.data_ptr() + 255) // 256 * 256
+            self.launch_ptrs(ins, outs, wptr, target)
         return outputs
 
     def close(self) -> None:

@@ -340,6 +340,36 @@ int32_t he_plan_conv2d(he_ctx* ctx, int32_t kind, const he_conv2d_params* params
                        int32_t in_w, int32_t dtype, const he_conv2d_fusion* fusion, he_plan** out);
 
 /* ------------------------------------------------------------------------------------------------
+ * Group normalisation with an activation over channels-last tensors: the normalisation of a convolutional net whose
+ * statistics do not tie a picture to its batch (the reference has batch norm only,
+ * helium/src/modules/batch_norm.rs:32-71; it composes anything else from reductions and pointwise ops).
+ * x is [batch, positions, channels] (NHWC with H and W flattened), dense; `groups` divides `channels`, a group is
+ * channels / groups neighbouring channels of one picture.  With mean and (biased) variance over a group's values,
+ *   rstd = 1 / sqrt(var + eps),  z = (x - mean) rstd gamma[c] + beta[c],  y = act(z).
+ *
+ * he_launch operands, in order:
+ *   HE_GN_FORWARD   inputs  x, gamma f32 [C], beta f32 [C]
+ *                   outputs y, mean f32 [batch, groups], rstd f32 [batch, groups]
+ *   HE_GN_BACKWARD  inputs  dy, x, gamma, beta, mean, rstd (the forward pass's)
+ *                   outputs dx, dgamma f32 [C], dbeta f32 [C] (summed over batch and positions)
+ * x, y, dy, dx have `dtype` (F16 / BF16 / F32), start on 16-byte boundaries and may not overlap one another where one is
+ * written; any sizes from one position and one channel on.  Sums and statistics are f32, taken in a fixed order: results
+ * repeat bit for bit.  The rectifier's derivative at 0 is 0.  A group that holds a NaN or an infinity comes out as NaN.
+ * ------------------------------------------------------------------------------------------------ */
+typedef enum he_activation { HE_ACT_NONE = 0, HE_ACT_RELU = 1, HE_ACT_SILU = 2, HE_ACT_GELU = 3 /* exact erf form */ } he_activation;
+typedef enum he_gn_direction { HE_GN_FORWARD = 0, HE_GN_BACKWARD = 1 } he_gn_direction;
+typedef struct he_group_norm_params {
+  int32_t batch;
+  int32_t channels;
+  int64_t positions;    /* H * W */
+  int32_t groups;
+  int32_t dtype;        /* of x, y, dy, dx */
+  int32_t activation;   /* he_activation */
+  float eps;            /* added to the variance */
+} he_group_norm_params;
+int32_t he_plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_params* params, he_plan** out);
+
+/* ------------------------------------------------------------------------------------------------
  * Hand-written kernels for the pointwise / reduction chains of a convolutional training step.  In the
  * reference each is a chain of generic pointwise and reduce instructions over broadcast views of
  * channels-last tensors; here each remaining pass over an activation is one HBM-bound kernel.  All tensors
