@@ -55,6 +55,14 @@ class HeGroupNormParams(C.Structure):
                 ("activation", C.c_int32), ("eps", C.c_float)]
 
 
+class HeMuonParams(C.Structure):
+    """struct he_muon_params of include/helium_b200.h."""
+
+    _fields_ = [("count", C.c_int32), ("rows", C.POINTER(C.c_int64)), ("cols", C.POINTER(C.c_int64)), ("scales", C.POINTER(C.c_float)),
+                ("grad_dtype", C.c_int32), ("out_dtype", C.c_int32), ("steps", C.c_int32), ("coef", C.c_float * 3), ("eps", C.c_float),
+                ("use_momentum", C.c_int32), ("momentum", C.c_float), ("nesterov", C.c_int32)]
+
+
 #: every symbol include/helium_b200.h declares: name -> (restype, argtypes)
 SIGNATURES = {
     "he_ctx_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
@@ -70,6 +78,7 @@ SIGNATURES = {
     "he_plan_conv2d": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(HeConv2dParams), C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                    C.POINTER(HeConv2dFusion), C.POINTER(C.c_void_p)]),
     "he_plan_group_norm": (C.c_int32, [C.c_void_p, C.c_int32, C.POINTER(HeGroupNormParams), C.POINTER(C.c_void_p)]),
+    "he_plan_muon": (C.c_int32, [C.c_void_p, C.POINTER(HeMuonParams), C.POINTER(C.c_void_p)]),
     "he_bn_finalize": (C.c_int32, [C.c_void_p, C.c_int64] + [C.c_void_p] * 8 + [C.c_int32, C.c_void_p]),
     "he_bn_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "he_bn_apply": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,

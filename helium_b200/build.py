@@ -40,6 +40,7 @@ SOURCES = [
     "conv.cu",
     "train_ops.cu",
     "group_norm.cu",
+    "muon.cu",
 ]
 
 NVCC_FLAGS = [

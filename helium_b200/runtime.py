@@ -13,7 +13,7 @@ from typing import List, Optional, Sequence
 import numpy as np
 
 from . import ir
-from ._abi import HeConv2dFusion, HeConv2dParams, HeGroupNormParams
+from ._abi import HeConv2dFusion, HeConv2dParams, HeGroupNormParams, HeMuonParams
 from ._lib import HeliumError, check, lib
 
 _TORCH_DTYPES = None
@@ -167,6 +167,29 @@ class Plan:
             plan = Plan(h, [x, (channels,), (channels,)], [dtype, ir.F32, ir.F32], 6, ctx)
             plan._in_specs = [(x, dtype), (x, dtype), ((channels,), ir.F32), ((channels,), ir.F32), ((batch, groups), ir.F32),
                               ((batch, groups), ir.F32)]
+        return plan
+
+    @staticmethod
+    def muon(ctx: Optional[Context], shapes: Sequence[tuple], grad_dtype: int = ir.BF16, out_dtype: int = ir.BF16,
+             momentum: Optional[float] = 0.95, nesterov: bool = True, steps: int = 5, coefs: Sequence[float] = (3.4445, -4.7750, 2.0315),
+             eps: float = 1e-7, scales: Optional[Sequence[float]] = None) -> "Plan":
+        """he_plan_muon for matrices of `shapes` [(rows, cols), ...].  Inputs: the gradients, then (unless `momentum` is
+        None) the f32 averages; outputs: the updates, then the new averages, which may be written over the old ones."""
+        n = len(shapes)
+        rows = (C.c_int64 * max(1, n))(*[s[0] for s in shapes])
+        cols = (C.c_int64 * max(1, n))(*[s[1] for s in shapes])
+        if scales is not None and len(scales) != n:
+            raise ValueError(f"{n} matrices, {len(scales)} scales")
+        sc = (C.c_float * max(1, n))(*scales) if scales is not None else None
+        m = 0.0 if momentum is None else momentum
+        prm = HeMuonParams(n, rows, cols, sc, grad_dtype, out_dtype, steps, (C.c_float * 3)(*coefs), eps, int(momentum is not None), m,
+                           int(nesterov))
+        h = C.c_void_p()
+        check(lib.he_plan_muon(ctx._h if ctx else None, C.byref(prm), C.byref(h)))
+        two = [tuple(s) for s in shapes]
+        avg = two if momentum is not None else []
+        plan = Plan(h, two + avg, [out_dtype] * n + [ir.F32] * len(avg), n + len(avg), ctx)
+        plan._in_specs = [(s, grad_dtype) for s in two] + [(s, ir.F32) for s in avg]
         return plan
 
     # -- queries -----------------------------------------------------------------------------------

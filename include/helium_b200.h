@@ -411,6 +411,36 @@ int32_t he_colsum_bf16(const void* x, float* out, void* workspace, int64_t pixel
  * step's convolutions read (helium/src/modules/conv.rs:63).  `avg` may be NULL for plain SGD (momentum 0). */
 int32_t he_sgd_momentum(float* w, float* avg, const void* grad, int32_t grad_dtype, void* w_bf16, int64_t n, float lr,
                         float momentum, int32_t first_step, void* cu_stream);
+/* The Muon optimiser's update for a list of weight matrices: each gradient's momentum average, orthogonalised by
+ * Newton-Schulz products on the tensor cores.  For every matrix (rows x cols, dense row-major; a convolution's filter
+ * [K,R,S,C] is K x RSC):
+ *   avg' = momentum avg + (1 - momentum) g          (helium's average, optimizer/sgd.rs:47-62; avg starts at zero)
+ *   d = nesterov ? momentum avg' + (1 - momentum) g : avg'     (use_momentum == 0: d = g)
+ *   X = d / (|d|_F + eps);  `steps` times:  X <- a X + (b S + c S^2) X  with S = X X^T  (X^T X where rows > cols)
+ *   update = scale X
+ * he_launch operands, in order:
+ *   inputs   gradient of every matrix (grad_dtype), then, with use_momentum, average of every matrix (f32)
+ *   outputs  update of every matrix (out_dtype: BF16 or F16), then, with use_momentum, the new averages (f32; an output
+ *            may be the input average itself, no other operands may overlap)
+ * The products run on f16 operands with f32 accumulation: an update is about 1e-3 (2-norm, relative) from the same steps in
+ * 64 bits; averages are f32.  `coef` must keep the singular values, which start in [0, 1], below 4.  The update is
+ * applied by he_sgd_momentum with `avg` NULL.  One workspace serves one launch at a time.  Tensors start on 16-byte
+ * boundaries; min(rows, cols) <= 32768. */
+typedef struct he_muon_params {
+  int32_t count;            /* matrices */
+  const int64_t* rows;      /* [count] */
+  const int64_t* cols;      /* [count] */
+  const float* scales;      /* [count] factor of each update; NULL: 1 */
+  int32_t grad_dtype;       /* F16 / BF16 / F32 */
+  int32_t out_dtype;        /* F16 / BF16 */
+  int32_t steps;
+  float coef[3];            /* a, b, c */
+  float eps;                /* added to the norm */
+  int32_t use_momentum;
+  float momentum;           /* [0, 1) */
+  int32_t nesterov;
+} he_muon_params;
+int32_t he_plan_muon(he_ctx* ctx, const he_muon_params* params, he_plan** out);
 /* Patch matrix of a 'Same'-padded convolution over a thin NHWC tensor (any channel count, e.g. RGB):
  * cols[n, p, q, (r * S + s) * C + c] = x[n, p * stride + r - R/2, q * stride + s - S/2, c], zero outside the image and
  * in the padding columns up to `pitch` (a multiple of 8).  The result, seen as an NHWC tensor with `pitch` channels,
