@@ -273,7 +273,8 @@ class Plan:
             target = torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream
         with torch.cuda.stream(target) if target != current else _NO_CONTEXT:
             if outputs is None:
-                outputs = self.alloc_outputs(inputs[0].device)
+                dev_t = inputs[0].device
+                outputs = [torch.empty(shape, dtype=_TORCH_DTYPES[dt], device=dev_t) for shape, dt in zip(self.out_shapes, self.out_dtypes)]
                 outs = [t.data_ptr() for t in outputs]
             else:
                 if len(outputs) != len(self.out_shapes):

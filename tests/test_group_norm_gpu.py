@@ -88,10 +88,11 @@ def _check_forward(plan, x, gamma, beta, groups, act, dt, y, mean, rstd, eps=EPS
 
 # (batch, positions, channels, groups): one position and one channel; channel counts that a 16-byte vector divides, meets
 # halfway and does not divide; positions that end inside a super-row; one group and a group per channel; more vector
-# columns than a CTA has threads; pictures of several slices
+# columns than a CTA has threads; pictures of several slices and pictures that a cluster's shared memory holds
 SIZES = [(1, 1, 1, 1), (3, 1, 5, 5), (2, 1, 512, 32), (1, 49, 512, 32), (4, 49, 64, 8), (5, 37, 60, 6), (3, 101, 77, 7), (7, 13, 3, 1),
          (2, 64, 24, 24), (3, 50, 320, 32), (1, 5000, 8, 1), (2, 777, 1, 1), (2, 9, 1023, 11), (1, 3, 8200, 8), (2, 4099, 96, 3),
-         (1, 70001, 40, 8), (2, 33000, 64, 32), (130, 6, 16, 2)]
+         (1, 70001, 40, 8), (2, 33000, 64, 32), (130, 6, 16, 2),
+         (2, 700001, 3, 1), (1, 120001, 77, 7), (2, 9001, 1023, 11), (1, 200000, 64, 8), (1, 5, 4096, 1), (2, 3, 2049, 3)]
 
 
 @pytest.mark.parametrize("dt", [ir.BF16, ir.F16, ir.F32])
