@@ -7,7 +7,7 @@
 //   update = scale X
 // so every singular value v of d / |d| is mapped by a v + b v^3 + c v^5 once per step.  helium builds optimisers from
 // pointwise ops and matmuls (helium/src/optimizer); the products here are three tcgen05 GEMMs a step over the whole list of
-// matrices at once, of which the symmetric ones (S and S^2) compute the tiles on and below the diagonal only.
+// matrices, of which the symmetric ones (S and S^2) compute the tiles on and below the diagonal only.
 //
 // Numbers.  The operands are f16, each matrix scaled by a power of two: X by sx ~ sqrt(m n), which makes its
 // root-mean-square 1 at the start and keeps |X| below 65504 (|X| <= 1.3 sx), S by 2^12, B by 2^10.  X itself is kept as a
@@ -26,7 +26,7 @@
 
 #include "device_utils.cuh"
 #include "he_internal.h"
-#include "sm100_ptx.cuh"
+#include "gemm_sm100_2cta.cuh"
 
 namespace he {
 namespace {
@@ -45,14 +45,24 @@ struct MuonMat {
   long long diag;              // first of m f32 values behind the table
   long long chunk;             // elements a CTA of the first pass sums
   int m, n, tall;              // m <= n; tall: the gradient is [n, m]
-  int mt, nt;                  // 128-row and 128-column tiles
+  int mt, nt;                  // 128-row and 128-column blocks (even numbers of them where CTA pairs work)
+  long long partial;           // first f32 of the split tiles of S (splits > 1)
   int part0, chunks;           // partial sums of squares
-  int sym0, x0, pack0;         // first tile of this matrix in the symmetric, product and packing grids
+  int s0, b0, x0, pack0;       // first item of this matrix in a step's list, first piece of the packing grid
+  int splits, split_blocks;    // S: slices of n, and 64-column blocks of one
+  int arrive0;                 // first arrival counter of the tiles of S
   float sx, out_scale;
 };
 struct MuonTable {
   int count;
+  int items_s, items_b, items; // of a step: the first phase, the first two, all three
   MuonMat mat[kMaxMats];
+};
+// Counters of a launch, zeroed by its first kernel; they only ever grow.
+struct MuonSync {
+  unsigned next;               // next item of the list
+  unsigned pad[31];
+  unsigned done[kMaxMats][4];  // tiles of S, B and X finished, by matrix, over all steps
 };
 struct MuonStep {
   float momentum, rest;        // m and 1 - m
@@ -86,11 +96,13 @@ __device__ __forceinline__ float direction(const MuonStep& st, float g, float av
 // ---- first pass: the average, and partial sums of squares of the direction ------------------------------------------
 // Squares are added in 64 bits: gradients as large as 1e30 and as small as 1e-25 keep their norm.
 __global__ void __launch_bounds__(kSumThreads) muon_average_kernel(const __grid_constant__ MuonTable t, const __grid_constant__ MuonStep st,
-                                                                  MuonTable* __restrict__ table_out, double* __restrict__ parts) {
+                                                                  MuonTable* __restrict__ table_out, double* __restrict__ parts,
+                                                                  unsigned* __restrict__ sync, int sync_words) {
   if (blockIdx.x == 0) {   // the later kernels read the table from memory
     const uint32_t* src = reinterpret_cast<const uint32_t*>(&t);
     uint32_t* dst = reinterpret_cast<uint32_t*>(table_out);
     for (int i = threadIdx.x; i < (int)(sizeof(MuonTable) / 4); i += kSumThreads) dst[i] = src[i];
+    for (int i = threadIdx.x; i < sync_words; i += kSumThreads) sync[i] = 0;
   }
   const int k = find_matrix(t.count, blockIdx.x, [&](int i) { return t.mat[i].part0; });
   const MuonMat& m = t.mat[k];
@@ -158,89 +170,158 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
 }
 
 // ---- second pass: the direction, scaled and split, into the blocks of the workspace; zeros behind its edges ----------
-__global__ void __launch_bounds__(256) muon_pack_kernel(const MuonTable* __restrict__ tp, const __grid_constant__ MuonStep st,
+// A CTA fills one block of 128 rows x 64 columns.  Where the gradient's rows run along X's and are whole vectors a thread
+// reads 8 columns and writes them; otherwise the block goes through shared memory, read along the gradient's own rows.
+__device__ __forceinline__ void load_grad8(const void* g, int dt, long long e, float (&v)[8]) {   // e * size is a multiple of 16
+  if (dt == HE_F32) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g) + e));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g) + e) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(g) + e));
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = dt == HE_BF16 ? bf16_bits_to_f32(w[i] & 0xffffu) : f16_bits_to_f32(w[i] & 0xffffu);
+      v[2 * i + 1] = dt == HE_BF16 ? bf16_bits_to_f32(w[i] >> 16) : f16_bits_to_f32(w[i] >> 16);
+    }
+  }
+}
+// the direction at 8 elements from e on
+__device__ __forceinline__ void direction8(const MuonMat& m, const MuonStep& st, long long e, float (&v)[8]) {
+  if (!st.has_momentum || st.nesterov) load_grad8(m.g, st.grad_dt, e, v);
+  if (st.has_momentum) {
+    const float4 a = *reinterpret_cast<const float4*>(m.avg_out + e), b = *reinterpret_cast<const float4*>(m.avg_out + e + 4);
+    const float av[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = direction(st, v[i], av[i]);
+  }
+}
+__device__ __forceinline__ float direction1(const MuonMat& m, const MuonStep& st, long long e) {
+  if (!st.has_momentum) return load_grad(m.g, st.grad_dt, e);
+  return direction(st, st.nesterov ? load_grad(m.g, st.grad_dt, e) : 0.0f, m.avg_out[e]);
+}
+constexpr int kPackPitch = 65;
+__global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ MuonTable t, const __grid_constant__ MuonStep st,
                                                         const double* __restrict__ parts, uint8_t* __restrict__ arena) {
-  __shared__ float tile[64][65];
-  __shared__ float scale_sh;
-  const MuonTable& t = *tp;
+  __shared__ float tile[kBlockRows * kPackPitch];
+  __shared__ double sums[8];
   const int k = find_matrix(t.count, blockIdx.x, [&](int i) { return t.mat[i].pack0; });
   const MuonMat& m = t.mat[k];
-  if (threadIdx.x < 32) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < m.chunks; i += 32) s += parts[m.part0 + i];
+  const int piece = blockIdx.x - m.pack0, cb = piece % (2 * m.nt), rb = piece / (2 * m.nt);
+  const int r0 = rb * kBlockRows, c0 = cb * kBlockCols;
+  // the norm, from the partial sums in a fixed order
+  double s = 0.0;
+  for (int i = threadIdx.x; i < m.chunks; i += 256) s += parts[m.part0 + i];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) scale_sh = (float)((double)m.sx / (sqrt(s) + (double)st.eps));
-  }
-  const int p = blockIdx.x - m.pack0, cb = p % (2 * m.nt), rb = p / (2 * m.nt);   // 64 x 64 piece
-  const int r0 = rb * 64, c0 = cb * 64;
-  __syncthreads();
-  const float scale = scale_sh;
-  // the gradient's own rows run along X's columns, or along its rows where it is tall
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int u = i >> 6, v = i & 63;
-    const int r = m.tall ? r0 + v : r0 + u, c = m.tall ? c0 + u : c0 + v;
-    float d = 0.0f;
-    if (r < m.m && c < m.n) {
-      const long long e = m.tall ? (long long)c * m.m + r : (long long)r * m.n + c;
-      if (!st.has_momentum) d = load_grad(m.g, st.grad_dt, e);
-      else d = st.nesterov ? direction(st, load_grad(m.g, st.grad_dt, e), m.avg_out[e]) : m.avg_out[e];
-      d *= scale;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
+  const bool direct = !m.tall && (m.n & 7) == 0, across = m.tall && (m.m & 7) == 0;
+  uint8_t* const hi_at = arena + (m.x[0] + x_block(m, rb, cb)) * 128;
+  uint8_t* const lo_at = arena + (m.xlo + x_block(m, rb, cb)) * 128;
+  if (!direct) {
+    if (across) {
+      for (int i = threadIdx.x; i < kBlockCols * 16; i += 256) {
+        const int c = i >> 4, r = (i & 15) * 8;
+        float v[8] = {};
+        if (c0 + c < m.n && r0 + r < m.m) direction8(m, st, (long long)(c0 + c) * m.m + r0 + r, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) tile[(r + q) * kPackPitch + c] = v[q];
+      }
+    } else {
+      for (int i = threadIdx.x; i < kBlockRows * kBlockCols; i += 256) {
+        const int r = m.tall ? i & 127 : i >> 6, c = m.tall ? i >> 7 : i & 63;
+        float d = 0.0f;
+        if (r0 + r < m.m && c0 + c < m.n)
+          d = direction1(m, st, m.tall ? (long long)(c0 + c) * m.m + r0 + r : (long long)(r0 + r) * m.n + c0 + c);
+        tile[r * kPackPitch + c] = d;
+      }
     }
-    tile[r - r0][c - c0] = d;
   }
   __syncthreads();
-  const long long row = x_block(m, r0 / kBlockRows, cb) + (r0 % kBlockRows);
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int r = i >> 3, q = (i & 7) * 8;
+  s = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
+  const float scale = (float)((double)m.sx / (sqrt(s) + (double)st.eps));
+#pragma unroll
+  for (int i = 0; i < kBlockRows * 8 / 256; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i, q = (threadIdx.x & 7) * 8;
+    float v[8] = {};
+    if (!direct) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = tile[r * kPackPitch + q + j];
+    } else if (r0 + r < m.m && c0 + q < m.n) {
+      direction8(m, st, (long long)(r0 + r) * m.n + c0 + q, v);
+    }
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair(tile[r][q + 2 * j], tile[r][q + 2 * j + 1], hi[j], lo[j]);
-    const long long at = (row + r) * 128 + q * 2;
-    *reinterpret_cast<uint4*>(arena + m.x[0] * 128 + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(arena + m.xlo * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    for (int j = 0; j < 4; ++j) split_pair(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+    *reinterpret_cast<uint4*>(hi_at + r * 128 + q * 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(lo_at + r * 128 + q * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
 // ---- the products -----------------------------------------------------------------------------------------------
+// One kernel for all steps.  The work is one list of items -- for every step the tiles of S, then of B, then of the new X,
+// each over all matrices -- and CTAs (or CTA pairs) take the next item from a counter.  An item waits for the counters of
+// its own matrix (S: the X of the step before is whole; B: S is; X: B is), which only items earlier in the list raise, and
+// those are in the hands of CTAs that run already: whatever the order and number of the CTAs, every wait ends.  A matrix's
+// phases follow one another without a launch or a grid-wide barrier between them, and other matrices fill the gaps.
+// The long sum of S (n columns, few tiles) is split into slices whose f32 tiles the last slice to arrive adds up, in the
+// order of the slices: results do not depend on who it was.
+//
+// PAIR = false: one CTA, 128 x 128 tiles.  PAIR = true: a cluster of two CTAs on 256 x 256 tiles (cta_group::2), each with
+// 128 rows and half of the column operand: half the bytes from L2 for the same products, which is what bounds 128 x 128
+// tiles (350 ns for the 32 KB of a 64-deep block, 13.5 TB/s over the chip, where the products take 140 ns).
+//
+// Warps: 0 items and loads, 1 products, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128 columns.  The tiles
+// that the epilogue reads (S, or X's two halves) follow a tile's operands through the same ring of stages, 64 columns a stage.
+// (Epilogue reads straight from L2, 64 bytes a lane, took 6 us a 128 x 128 tile; two teams on tiles that TMA brought took 3.5
+// us, their few warps waiting for their own arithmetic.)
 enum Phase { PH_S = 0, PH_B = 1, PH_X = 2 };
 constexpr int kTile = 128, kKBlock = 64;
-constexpr int kStages = 3;                                  // 96 KB: two CTAs fit an SM, one's epilogue under the other's products
+constexpr int kStages = 6;
 constexpr int kOperandBytes = kTile * kKBlock * 2;          // 16 KB
-constexpr int kGemmThreads = 192;                           // producer warp, MMA warp, four epilogue warps
-constexpr int kGemmSmem = kStages * 2 * kOperandBytes + (2 * kStages + 2) * 8 + 16 + 1024;
+constexpr int kEpiThreads = 512;
+constexpr int kGemmThreads = 128 + kEpiThreads;
+constexpr int kSlots = 4;                                   // items in flight in a CTA
 
-struct GemmArgs {
+struct Item {
+  int phase, mat, i, j, k0, k_blocks, split, step;
+};
+struct IterShared {
+  MuonTable table;
+  Item item[kSlots];
+  uint64_t full[kStages], empty[kStages], item_full[kSlots], item_empty[kSlots], acc_full[2], acc_empty[2], epi_full[kSlots][4], drain;
+  uint32_t tmem;
+  int abort_flag;
+  int last_split;
+  unsigned short stage[kEpiThreads / 32][32][18];   // a warp's 32 x 16 outputs
+};
+constexpr int kOffShared = kStages * 2 * kOperandBytes;
+constexpr int kIterSmem = kOffShared + (int)sizeof(IterShared) + 1024;
+static_assert(kIterSmem <= 232448, "shared memory budget of sm_100 exceeded");
+
+struct IterArgs {
   const MuonTable* table;
+  MuonSync* sync;
+  unsigned* arrive;  // a counter for every tile of S and CTA of its pair
   uint8_t* arena;
   float* diag;
+  float* partial;
   DeviceStatus* status;
   unsigned wait_limit_us;
   int withhold_loads;
-  int cur;           // buffer of X that the step reads
-  int last;          // the step writes the update
-  float b, c, a;
+  int steps;
+  float a, b, c;
   int out_dt;
 };
 
-// 64 bytes; not through the read-only path, since the lo values are rewritten in place by the thread that read them
-__device__ __forceinline__ void load_chunk(const uint8_t* p, uint32_t (&w)[16]) {
+// 16 columns of row r (c0 a multiple of 16) of a 128 x 64 block in shared memory, 128-byte swizzle
+__device__ __forceinline__ void load_block_row(const uint8_t* block, int r, int c0, uint32_t (&w)[8]) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(w[8 * h]), "=r"(w[8 * h + 1]), "=r"(w[8 * h + 2]), "=r"(w[8 * h + 3]), "=r"(w[8 * h + 4]), "=r"(w[8 * h + 5]),
-                   "=r"(w[8 * h + 6]), "=r"(w[8 * h + 7])
-                 : "l"(p + 32 * h)
-                 : "memory");
-}
-__device__ __forceinline__ void store_chunk(uint8_t* p, const uint32_t (&w)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = w[i];
-  ptx::st_global_256(p, r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = w[8 + i];
-  ptx::st_global_256(p + 32, r);
+  for (int h = 0; h < 2; ++h) {
+    const uint4 v = *reinterpret_cast<const uint4*>(block + r * 128 + ((((c0 >> 3) + h) ^ (r & 7)) << 4));
+    w[4 * h] = v.x; w[4 * h + 1] = v.y; w[4 * h + 2] = v.z; w[4 * h + 3] = v.w;
+  }
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -250,215 +331,517 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 __device__ __forceinline__ unsigned short out_bits(float v, int dt) {
   return (unsigned short)(dt == HE_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
 }
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+// orders what was acquired before it against this thread's TMA loads
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 
-template <int PH>
-__global__ void __launch_bounds__(kGemmThreads) muon_gemm_kernel(const __grid_constant__ CUtensorMap map128,
-                                                                 const __grid_constant__ CUtensorMap map64, const __grid_constant__ GemmArgs p) {
+// Waits until *p >= want.  Bounded like every wait here.
+__device__ __forceinline__ bool wait_count(const unsigned* p, unsigned want, volatile int* abort_flag, DeviceStatus* status, uint32_t limit_us) {
+  if (load_acquire(p) >= want) return true;
+  const uint64_t t0 = ptx::globaltimer_ns();
+  while (load_acquire(p) < want) {
+    if (*abort_flag) return false;
+    if (ptx::globaltimer_ns() - t0 > (uint64_t)limit_us * 1000ull) {
+      *abort_flag = 1;
+      if (status && atomicCAS(&status->code, 0u, (9u << 16) | (want & 0xffffu)) == 0u) { status->block = blockIdx.x; status->aux0 = want; }
+      return false;
+    }
+  }
+  return true;
+}
+
+// Named barrier of `threads` threads that tells each of them whether all of them said yes.
+__device__ __forceinline__ bool barrier_all(uint32_t id, uint32_t threads, bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)yes)
+      : "memory");
+  return r != 0;
+}
+
+template <bool PAIR> __device__ __forceinline__ Item decode_item(const MuonTable& t, unsigned id, int steps) {
+  Item w;
+  w.step = (int)(id / (unsigned)t.items);
+  if (w.step >= steps) { w.phase = -1; return w; }
+  const int r = (int)(id - (unsigned)w.step * (unsigned)t.items);
+  w.phase = r < t.items_s ? PH_S : r < t.items_b ? PH_B : PH_X;
+  const int phase = w.phase;
+  w.mat = find_matrix(t.count, r, [&](int q) { return phase == PH_S ? t.mat[q].s0 : phase == PH_B ? t.mat[q].b0 : t.mat[q].x0; });
+  const MuonMat& m = t.mat[w.mat];
+  w.split = 0;
+  w.k0 = 0;
+  w.k_blocks = (m.m + kKBlock - 1) / kKBlock;
+  if (phase == PH_X) {
+    const int q = r - m.x0, ti = PAIR ? m.mt >> 1 : m.mt;
+    w.j = q / ti;        // neighbours in the list share X's columns
+    w.i = q - w.j * ti;
+    return w;
+  }
+  int q = r - (phase == PH_S ? m.s0 : m.b0);
+  if (phase == PH_S) {
+    w.k_blocks = (m.n + kKBlock - 1) / kKBlock;
+    if (m.splits > 1) {
+      w.split = q % m.splits;
+      q /= m.splits;
+      w.k0 = w.split * m.split_blocks;
+      w.k_blocks = min(m.split_blocks, w.k_blocks - w.k0);
+    }
+  }
+  w.i = (int)((sqrtf(8.0f * q + 1.0f) - 1.0f) * 0.5f);
+  while ((w.i + 1) * (w.i + 2) / 2 <= q) ++w.i;
+  while (w.i * (w.i + 1) / 2 > q) --w.i;
+  w.j = q - w.i * (w.i + 1) / 2;
+  return w;
+}
+
+// store to the same place of CTA `rank`'s shared memory
+__device__ __forceinline__ void store_peer(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void arrive_peer_release(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ void fence_cluster_acquire() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+
+template <bool PAIR>
+__global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __grid_constant__ CUtensorMap map128,
+                                                                       const __grid_constant__ CUtensorMap map64,
+                                                                       const __grid_constant__ IterArgs p) {
+  constexpr int kN = PAIR ? 256 : 128;        // columns of a tile
+  constexpr int kGroups = kN / 64;
+  constexpr int kCtas = PAIR ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  IterShared& sh = *reinterpret_cast<IterShared*>(smem + kOffShared);
   const uint32_t base = ptx::smem_u32(smem);
-  const uint32_t bars = base + kStages * 2 * kOperandBytes;
-  auto bar_full = [&](int s) { return bars + 8u * s; };
-  auto bar_empty = [&](int s) { return bars + 8u * (kStages + s); };
-  const uint32_t bar_done = bars + 8u * (2 * kStages), bar_drain = bar_done + 8u;
-  volatile uint32_t* tmem_holder = reinterpret_cast<volatile uint32_t*>(smem + kStages * 2 * kOperandBytes + (2 * kStages + 2) * 8);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  auto bar = [](uint64_t& b) { return ptx::smem_u32(&b); };
+  volatile int* abort_flag = &sh.abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // the tile: row block i, column block j (the symmetric products: j <= i)
-  const MuonTable& t = *p.table;
-  const int mi = find_matrix(t.count, blockIdx.x, [&](int q) { return PH == PH_X ? t.mat[q].x0 : t.mat[q].sym0; });
-  const MuonMat& m = t.mat[mi];
-  int i, j;
-  if (PH == PH_X) {
-    const int q = blockIdx.x - m.x0;
-    j = q / m.mt;      // neighbours share X's columns
-    i = q - j * m.mt;
-  } else {
-    const int q = blockIdx.x - m.sym0;
-    i = (int)((sqrtf(8.0f * q + 1.0f) - 1.0f) * 0.5f);
-    while ((i + 1) * (i + 2) / 2 <= q) ++i;
-    while (i * (i + 1) / 2 > q) --i;
-    j = q - i * (i + 1) / 2;
-  }
-  const bool same = PH != PH_X && i == j;    // both operands are one block row: loaded once
-  const int k_blocks = PH == PH_S ? (m.n + kKBlock - 1) / kKBlock : (m.m + kKBlock - 1) / kKBlock;
+  const uint32_t rank = PAIR ? ptx::cluster_ctarank() : 0u;
+  const bool leader = rank == 0;
+  // a barrier of the leader, seen from either CTA
+  auto lead = [&](uint64_t& b) { return PAIR ? ptx::mapa(bar(b), 0) : bar(b); };
+  auto arrive_lead = [&](uint64_t& b) {
+    if (PAIR) ptx::mbar_arrive_cluster(ptx::mapa(bar(b), 0));
+    else ptx::mbar_arrive(bar(b));
+  };
 
   if (threadIdx.x == 0) {
-    *abort_flag = 0;
-    for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(bar_full(s), 1);
-      ptx::mbar_init(bar_empty(s), 1);
+    sh.abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) { ptx::mbar_init(bar(sh.full[s]), 1); ptx::mbar_init(bar(sh.empty[s]), 1); }
+    for (int s = 0; s < kSlots; ++s) { ptx::mbar_init(bar(sh.item_full[s]), 1); ptx::mbar_init(bar(sh.item_empty[s]), kCtas * (kEpiThreads / 32)); }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(bar(sh.acc_full[s]), 1);
+      ptx::mbar_init(bar(sh.acc_empty[s]), kCtas * (kEpiThreads / 32));
     }
-    ptx::mbar_init(bar_done, 1);
-    ptx::mbar_init(bar_drain, 1);
+    for (int s = 0; s < kSlots * 4; ++s) ptx::mbar_init(bar(sh.epi_full[s >> 2][s & 3]), 1);
+    ptx::mbar_init(bar(sh.drain), 1);
     ptx::fence_mbar_init();
   }
   if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_holder)), kTile);
-    ptx::tmem_relinquish();
+    if (PAIR) {
+      ptx::tmem_alloc_2cta(ptx::smem_u32(&sh.tmem), 2 * kN);
+      ptx::tmem_relinquish_2cta();
+    } else {
+      ptx::tmem_alloc(ptx::smem_u32(&sh.tmem), 2 * kN);
+      ptx::tmem_relinquish();
+    }
+  }
+  {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.table);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(&sh.table);
+    const int words = (int)((sizeof(MuonTable) - sizeof(MuonMat) * (kMaxMats - p.table->count)) / 4);
+    for (int i = threadIdx.x; i < words; i += kGemmThreads) dst[i] = src[i];
   }
   ptx::tcgen05_fence_before();
   __syncthreads();
+  if (PAIR) ptx::cluster_sync();
   ptx::tcgen05_fence_after();
-  const uint32_t tmem = *tmem_holder;
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  const MuonTable& t = sh.table;
 
   if (warp == 0) {
-    if (lane == 0 && !p.withhold_loads) {
-      int kb = 0;
+    // ===================== items and operand loads =====================
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      unsigned filled = 0, any = 0;                  // operand fills of each stage: parity, and whether there were any
+      unsigned epi_filled = 0, epi_any = 0;          // the same of each epilogue barrier
+      const uint32_t full0 = bar(sh.full[0]), empty0 = bar(sh.empty[0]);
+      auto bar_full = [&](int s) { return full0 + 8u * s; };
+      auto bar_empty = [&](int s) { return empty0 + 8u * s; };
+      DeviceStatus* const status = p.status;
+      const uint32_t wait_us = p.wait_limit_us;
       bool alive = true;
-      for (; kb < k_blocks; ++kb) {
-        const int s = kb % kStages;
-        const uint32_t ph = (uint32_t)(kb / kStages) & 1u;
-        if (!ptx::mbar_wait(bar_empty(s), ph ^ 1u, abort_flag, p.status, 1, s, p.wait_limit_us)) { alive = false; break; }
-        const uint32_t a_dst = base + s * 2 * kOperandBytes, b_dst = a_dst + kOperandBytes;
-        ptx::mbar_arrive_expect_tx(bar_full(s), same ? kOperandBytes : 2 * kOperandBytes);
-        if (PH == PH_S) {
-          ptx::tma_load_3d(a_dst, &map128, bar_full(s), 0, (int)(m.x[p.cur] + x_block(m, i, kb)), 0);
-          if (!same) ptx::tma_load_3d(b_dst, &map128, bar_full(s), 0, (int)(m.x[p.cur] + x_block(m, j, kb)), 0);
-        } else if (PH == PH_B) {
-          ptx::tma_load_3d(a_dst, &map128, bar_full(s), 0, (int)(m.s + s_block(m, i, kb)), 0);
-          if (!same) ptx::tma_load_3d(b_dst, &map128, bar_full(s), 0, (int)(m.s + s_block(m, j, kb)), 0);
-        } else {
-          ptx::tma_load_3d(a_dst, &map128, bar_full(s), 0, (int)(m.b + s_block(m, i, kb)), 0);
+      for (int n = 0; alive; ++n) {
+        const int slot = n % kSlots;
+        Item w;
+        if (leader) {
+          // taken when the loads of the one before are out, no earlier: a CTA that waits must not sit on a second item
+          w = decode_item<PAIR>(t, atomicAdd(&p.sync->next, 1u), p.steps);
+          if (!ptx::mbar_wait(bar(sh.item_empty[slot]), ((uint32_t)(n / kSlots) & 1u) ^ 1u, abort_flag, p.status, 1, slot, p.wait_limit_us)) { alive = false; break; }
+          if (w.phase >= 0) {
+            const MuonMat& m = t.mat[w.mat];
+            const unsigned* done = p.sync->done[w.mat];
+            const unsigned ti = (unsigned)(PAIR ? m.mt >> 1 : m.mt), tj = (unsigned)(PAIR ? m.nt >> 1 : m.nt), sym = ti * (ti + 1) / 2 * kCtas;
+            if (w.phase == PH_S) alive = wait_count(done + PH_X, (unsigned)w.step * ti * tj * kCtas, abort_flag, p.status, p.wait_limit_us);
+            else alive = wait_count(done + (w.phase == PH_B ? PH_S : PH_B), (unsigned)(w.step + 1) * sym, abort_flag, p.status, p.wait_limit_us);
+            if (!alive) break;
+          }
+          sh.item[slot] = w;
+          if (PAIR) {
+            const uint32_t peer = ptx::mapa(ptx::smem_u32(&sh.item[slot]), 1);
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(&w);
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            ptx::tma_load_3d(b_dst + h * (kOperandBytes / 2), &map64, bar_full(s), 0,
-                             (int)(m.x[p.cur] + x_block(m, kb >> 1, 2 * j + h) + (kb & 1) * 64), 0);
+            for (int i = 0; i < (int)(sizeof(Item) / 4); ++i) store_peer(peer + 4 * i, words[i]);
+            arrive_peer_release(ptx::mapa(bar(sh.item_full[slot]), 1));
+          }
+          ptx::mbar_arrive(bar(sh.item_full[slot]));
+        } else {
+          if (!ptx::mbar_wait(bar(sh.item_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, p.status, 3, slot, 2 * p.wait_limit_us)) { alive = false; break; }
+          fence_cluster_acquire();
+          w = sh.item[slot];
+        }
+        if (w.phase < 0) break;
+        fence_proxy_async_all();
+        if (p.withhold_loads) continue;
+        const MuonMat& m = t.mat[w.mat];
+        const bool same = w.phase != PH_X && w.i == w.j;   // both operands are one block row: loaded once
+        const int ri = PAIR ? 2 * w.i + (int)rank : w.i, rj = PAIR ? 2 * w.j + (int)rank : w.j;
+        const int xcur = (int)m.x[w.step & 1], x_pitch = 2 * m.nt * kBlockRows, s_pitch = 2 * m.mt * kBlockRows;
+        // Rows of the arena that the next block of each operand starts at.  One thread paces the ring: what it computes for
+        // a block is two additions (with the addresses worked out from the tile each time a block took 350 ns).
+        int row_a = (w.phase == PH_S ? xcur + ri * x_pitch : (w.phase == PH_B ? (int)m.s : (int)m.b) + ri * s_pitch) + w.k0 * kBlockRows;
+        int row_b = w.phase == PH_S ? xcur + rj * x_pitch + w.k0 * kBlockRows : w.phase == PH_B ? (int)m.s + rj * s_pitch : xcur + 2 * rj * kBlockRows;
+        const uint32_t bytes = (same ? 1 : 2) * kCtas * kOperandBytes;
+        auto fill = [&](auto load_b) {
+          for (int kb = 0; kb < w.k_blocks; ++kb) {
+            if (!ptx::mbar_wait(bar_empty(stage), phase ^ 1u, abort_flag, status, 2, stage, wait_us)) { alive = false; break; }
+            const uint32_t a_dst = base + stage * 2 * kOperandBytes, fb = PAIR ? ptx::mapa(bar_full(stage), 0) : bar_full(stage);
+            if (leader) ptx::mbar_arrive_expect_tx(bar_full(stage), bytes);
+            filled ^= 1u << stage;
+            any |= 1u << stage;
+            if (PAIR) ptx::tma_load_3d_2cta(a_dst, &map128, fb, 0, row_a, 0);
+            else ptx::tma_load_3d(a_dst, &map128, fb, 0, row_a, 0);
+            load_b(a_dst + kOperandBytes, fb, kb);
+            row_a += kBlockRows;
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          }
+        };
+        if (w.phase == PH_X) {
+          fill([&](uint32_t dst, uint32_t fb, int kb) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (PAIR) ptx::tma_load_3d_2cta(dst + h * (kOperandBytes / 2), &map64, fb, 0, row_b + h * kBlockRows, 0);
+              else ptx::tma_load_3d(dst + h * (kOperandBytes / 2), &map64, fb, 0, row_b + h * kBlockRows, 0);
+            }
+            row_b += kb & 1 ? x_pitch - 64 : 64;    // X's rows, 64 at a time
+          });
+        } else {
+          fill([&](uint32_t dst, uint32_t fb, int) {
+            if (!same) {
+              if (PAIR) ptx::tma_load_3d_2cta(dst, &map128, fb, 0, row_b, 0);
+              else ptx::tma_load_3d(dst, &map128, fb, 0, row_b, 0);
+            }
+            row_b += kBlockRows;
+          });
+        }
+        if (w.phase == PH_S || !alive) continue;
+        // the epilogue's tiles, each CTA its own rows
+        int row = (w.phase == PH_X ? xcur + ri * x_pitch : (int)m.s + ri * s_pitch) + kGroups * w.j * kBlockRows;
+        const int lo = (int)m.xlo - xcur;
+        for (int g = 0; g < kGroups; ++g, row += kBlockRows) {
+          if (!ptx::mbar_wait(bar_empty(stage), phase ^ 1u, abort_flag, status, 2, stage, wait_us)) { alive = false; break; }
+          const uint32_t dst = base + stage * 2 * kOperandBytes, eb = bar(sh.epi_full[slot][g]);
+          ptx::mbar_arrive_expect_tx(eb, (w.phase == PH_X ? 2 : 1) * kOperandBytes);
+          ptx::tma_load_3d(dst, &map128, eb, 0, row, 0);
+          if (w.phase == PH_X) ptx::tma_load_3d(dst + kOperandBytes, &map128, eb, 0, row + lo, 0);
+          epi_filled ^= 1u << (4 * slot + g);
+          epi_any |= 1u << (4 * slot + g);
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      // a tile that was given up: the copies in flight still land in this CTA's memory
-      if (!alive)
-        for (int b = kb > kStages ? kb - kStages : 0; b < kb; ++b) {
-          int never = 0;
-          ptx::mbar_wait(bar_full(b % kStages), (uint32_t)(b / kStages) & 1u, &never, p.status, 7, b % kStages, p.wait_limit_us);
-        }
+      // an item that was given up: the copies in flight still land in this CTA's memory (the operands' count is the leader's)
+      if (!alive) {
+        int never = 0;
+        if (leader)
+          for (int s = 0; s < kStages; ++s)
+            if (any >> s & 1u) ptx::mbar_wait(bar(sh.full[s]), (filled >> s & 1u) ^ 1u, &never, p.status, 7, s, p.wait_limit_us);
+        for (int k = 0; k < kSlots * 4; ++k)
+          if (epi_any >> k & 1u) ptx::mbar_wait(bar(sh.epi_full[k >> 2][k & 3]), (epi_filled >> k & 1u) ^ 1u, &never, p.status, 11, k, p.wait_limit_us);
+      }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr bool kBMn = PH == PH_X;
-      const uint32_t idesc = ptx::make_idesc_f16(0, 0, kBMn ? 1 : 0, kTile, kTile);
-      constexpr uint32_t b_lbo = kBMn ? kOperandBytes / 2 : 16, b_kadv = kBMn ? 2048 : 32;
+    // ===================== products =====================
+    if (lane == 0 && leader) {
+      int stage = 0;
+      unsigned full_parity = 0;      // bit s: parity of the next operand fill of stage s (tiles of the epilogue fill others)
+      const uint32_t full0 = bar(sh.full[0]), empty0 = bar(sh.empty[0]), empty1 = PAIR ? ptx::mapa(empty0, 1) : 0u;
+      DeviceStatus* const status = p.status;
+      const uint32_t wait_us = p.wait_limit_us;
+      const uint64_t a_desc0 = ptx::make_smem_desc_sw128(base, 16, 1024);
       bool alive = true;
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        const int s = kb % kStages;
-        if (!ptx::mbar_wait(bar_full(s), (uint32_t)(kb / kStages) & 1u, abort_flag, p.status, 3, s, p.wait_limit_us)) { alive = false; break; }
+      for (int n = 0; alive; ++n) {
+        const int slot = n % kSlots, acc = n & 1;
+        if (!ptx::mbar_wait(bar(sh.item_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, status, 3, slot, 2 * wait_us)) { alive = false; break; }
+        const int phase = sh.item[slot].phase, k_blocks = sh.item[slot].k_blocks;
+        if (phase < 0) break;
+        const bool same = phase != PH_X && sh.item[slot].i == sh.item[slot].j;
+        if (!ptx::mbar_wait(bar(sh.acc_empty[acc]), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_flag, status, 4, acc, wait_us)) { alive = false; break; }
         ptx::tcgen05_fence_after();
-        const uint32_t a_addr = base + s * 2 * kOperandBytes, b_addr = same ? a_addr : a_addr + kOperandBytes;
+        const bool b_mn = phase == PH_X;
+        const uint32_t idesc = ptx::make_idesc_f16(0, 0, b_mn ? 1 : 0, kCtas * kTile, kN);
+        // descriptors of stage 0; a stage, and 16 values of k within it, are additions to the address field
+        const uint64_t b_desc0 = ptx::make_smem_desc_sw128(base + (same ? 0 : kOperandBytes), b_mn ? kOperandBytes / 2 : 16, 1024);
+        const uint32_t b_step = b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t d = tmem + (uint32_t)(acc * kN);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!ptx::mbar_wait(full0 + 8u * stage, full_parity >> stage & 1u, abort_flag, status, 5, stage, wait_us)) { alive = false; break; }
+          full_parity ^= 1u << stage;
+          ptx::tcgen05_fence_after();
+          const uint64_t ad = a_desc0 + (uint32_t)(stage * (2 * kOperandBytes >> 4)), bd = b_desc0 + (uint32_t)(stage * (2 * kOperandBytes >> 4));
 #pragma unroll
-        for (int k = 0; k < kKBlock / 16; ++k)
-          ptx::umma_f16(tmem, ptx::make_smem_desc_sw128(a_addr + k * 32, 16, 1024), ptx::make_smem_desc_sw128(b_addr + k * b_kadv, b_lbo, 1024),
-                        idesc, (kb | k) != 0 ? 1u : 0u);
-        ptx::umma_commit(bar_empty(s));
+          for (int k = 0; k < kKBlock / 16; ++k) {
+            if (PAIR) ptx::umma_f16_2cta(d, ad + 2 * k, bd + b_step * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            else ptx::umma_f16(d, ad + 2 * k, bd + b_step * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          if (PAIR) {
+            ptx::umma_commit_2cta(empty0 + 8u * stage);
+            ptx::umma_commit_2cta(empty1 + 8u * stage);
+          } else {
+            ptx::umma_commit(empty0 + 8u * stage);
+          }
+          if (++stage == kStages) stage = 0;
+        }
+        if (phase != PH_S) stage = (stage + kGroups) % kStages;   // the epilogue's tiles
+        if (alive) {
+          if (PAIR) {
+            ptx::umma_commit_2cta(bar(sh.acc_full[acc]));
+            ptx::umma_commit_2cta(ptx::mapa(bar(sh.acc_full[acc]), 1));
+          } else {
+            ptx::umma_commit(bar(sh.acc_full[acc]));
+          }
+        }
       }
-      ptx::umma_commit(alive ? bar_done : bar_drain);
       if (!alive) {   // nothing may still write tensor memory when it is freed
         int never = 0;
-        ptx::mbar_wait(bar_drain, 0, &never, p.status, 8, 0, p.wait_limit_us);
+        if (PAIR) ptx::umma_commit_2cta(bar(sh.drain));
+        else ptx::umma_commit(bar(sh.drain));
+        ptx::mbar_wait(bar(sh.drain), 0, &never, p.status, 8, 0, p.wait_limit_us);
       }
     }
-  } else {
-    const bool ok = ptx::mbar_wait(bar_done, 0, abort_flag, p.status, 4, 0, p.wait_limit_us);
-    if (__all_sync(0xffffffffu, ok)) {
+  } else if (warp >= 4) {
+    // ===================== epilogue: thread = row of the tile, team = 32 columns of every 128 =====================
+    const int quadrant = warp & 3, team = (warp - 4) >> 2, buf = team >> 1, r = quadrant * 32 + lane;
+    const int tid = threadIdx.x - 128;
+    int first_stage = 0;           // of the item
+    unsigned epi_parity = 0;       // of the next fill of each epilogue barrier
+    for (int n = 0;; ++n) {
+      const int slot = n % kSlots, acc = n & 1;
+      // the warps go on or give up together: they share barriers below
+      bool ok = ptx::mbar_wait(bar(sh.item_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, p.status, 3, slot, 2 * p.wait_limit_us);
+      if (PAIR) fence_cluster_acquire();
+      const Item w = sh.item[slot];
+      const int ri = PAIR ? 2 * w.i + (int)rank : w.i;   // block row of this CTA
+      const int grow = ri * kTile + r;
+      float dg = 0.0f;         // of this row, while the products run
+      if (ok && w.phase == PH_X) dg = p.a + __ldcg(p.diag + t.mat[w.mat].diag + grow);
+      if (ok && w.phase >= 0) ok = ptx::mbar_wait(bar(sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u, abort_flag, p.status, 6, acc, p.wait_limit_us);
+      if (!barrier_all(1, kEpiThreads, ok && w.phase >= 0)) break;
       ptx::tcgen05_fence_after();
-      const int quadrant = warp & 3, r = quadrant * 32 + lane;
-      const int grow = i * kTile + r;
-      const float inv_x2 = kScaleS / (m.sx * m.sx);
-      float dg = 0.0f;
-      if (PH == PH_X) dg = p.a + p.diag[m.diag + grow];
+      const MuonMat& m = t.mat[w.mat];
+      const uint32_t taddr = tmem + ((uint32_t)(quadrant * 32) << 16) + (uint32_t)(acc * kN);
+      auto release = [&]() {   // the accumulator
+        ptx::tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_lead(sh.acc_empty[acc]);
+      };
+      bool finish = true;      // this CTA completes the tile
+      const bool split = w.phase == PH_S && m.splits > 1;
+      float* part = nullptr;
+      if (split) {
+        // slices side by side, each [column][row]
+        const int tile = (w.i * (w.i + 1) / 2 + w.j) * kCtas + (int)rank;
+        part = p.partial + m.partial + (size_t)tile * m.splits * (kTile * kN);
+        float* mine = part + (size_t)w.split * (kTile * kN) + r;
 #pragma unroll 1
-      for (int c0 = 0; c0 < kTile; c0 += 32) {
-        uint32_t acc[32];
-        ptx::tmem_ld_32x32(tmem + ((uint32_t)(quadrant * 32) << 16) + (uint32_t)c0, acc);
-        // this thread's 32 columns in block (i, 2 j + c0 / 64): 64 bytes
-        const long long sym_at = (s_block(m, i, 2 * j + (c0 >> 6)) + r) * 128 + (c0 & 32) * 2;
-        const long long x_at = (x_block(m, i, 2 * j + (c0 >> 6)) + r) * 128 + (c0 & 32) * 2;
-        uint32_t w0[16], w1[16];
-        if (PH == PH_B) load_chunk(p.arena + m.s * 128 + sym_at, w0);
-        if (PH == PH_X) {
-          load_chunk(p.arena + m.x[p.cur] * 128 + x_at, w0);
-          load_chunk(p.arena + m.xlo * 128 + x_at, w1);
+        for (int c0 = team * 32; c0 < kN; c0 += 128) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(taddr + (uint32_t)c0, v);
+          ptx::tmem_ld_wait_regs(v);
+#pragma unroll
+          for (int q = 0; q < 32; ++q) mine[(c0 + q) * kTile] = __uint_as_float(v[q]);
         }
-        ptx::tmem_ld_wait_regs(acc);
-        float v[32];
-#pragma unroll
-        for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(acc[q]);
-        if (PH == PH_S) {
-#pragma unroll
-          for (int q = 0; q < 32; ++q) v[q] *= inv_x2;
-        } else if (PH == PH_B) {
-          const float kb = p.b * (kScaleB / kScaleS), kc = p.c * (kScaleB / (kScaleS * kScaleS));
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 s = unpack_half2(w0[q]);
-            v[2 * q] = fmaf(kc, v[2 * q], kb * s.x);
-            v[2 * q + 1] = fmaf(kc, v[2 * q + 1], kb * s.y);
-          }
-          if (i == j) {   // the diagonal stays f32
-#pragma unroll
-            for (int q = 0; q < 32; ++q)
-              if (c0 + q == r) {
-                p.diag[m.diag + grow] = v[q] * (1.0f / kScaleB);
-                v[q] = 0.0f;
-              }
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 h = unpack_half2(w0[q]), l = unpack_half2(w1[q]);
-            v[2 * q] = fmaf(dg, h.x + l.x, v[2 * q] * (1.0f / kScaleB));
-            v[2 * q + 1] = fmaf(dg, h.y + l.y, v[2 * q + 1] * (1.0f / kScaleB));
-          }
+        release();
+        ptx::named_barrier_sync(1, kEpiThreads);
+        if (tid == 0) {
+          __threadfence();
+          const unsigned before = atomicAdd(p.arrive + m.arrive0 + tile, 1u);
+          sh.last_split = (before + 1) % (unsigned)m.splits == 0;
+          __threadfence();
         }
-        if (PH != PH_X) {
-          uint8_t* dst = p.arena + (PH == PH_S ? m.s : m.b) * 128;
-#pragma unroll
-          for (int q = 0; q < 16; ++q) w0[q] = pack_half2(v[2 * q], v[2 * q + 1]);
-          store_chunk(dst + sym_at, w0);
-          if (i != j) {   // the mirrored tile: lanes are neighbouring columns of it
-            unsigned short* mir = reinterpret_cast<unsigned short*>(dst + (s_block(m, j, 2 * i + (r >> 6)) + c0) * 128) + (r & 63);
-#pragma unroll
-            for (int q = 0; q < 32; ++q) mir[q * 64] = (unsigned short)(w0[q >> 1] >> (16 * (q & 1)));
+        ptx::named_barrier_sync(1, kEpiThreads);
+        finish = sh.last_split != 0;
+      }
+      if (finish) {
+        const bool last = w.step == p.steps - 1;
+        const int cur = w.step & 1;
+        const float s_scale = kScaleS / (m.sx * m.sx), o_scale = m.out_scale / m.sx;
+#pragma unroll 1
+        for (int g = buf; g < kGroups; g += 2) {
+          const int cb = kGroups * w.j + g;       // 64-column block of the matrix
+          const int stage = (first_stage + w.k_blocks + g) % kStages;
+          const uint8_t* const epi = smem + stage * 2 * kOperandBytes;
+          if (w.phase != PH_S) {
+            // (a wait that runs out leaves stale values behind, and the abort flag: the item loop ends at its next wait)
+            const int k = 4 * slot + g;
+            ptx::mbar_wait(bar(sh.epi_full[slot][g]), epi_parity >> k & 1u, abort_flag, p.status, 12, k, p.wait_limit_us);
+            epi_parity ^= 1u << k;
+            __syncwarp();
           }
-        } else if (!p.last) {
+#pragma unroll 1
+          for (int c0 = (team & 1) * 32, half = 0; half < 2; ++half, c0 += 16) {
+            float v[16];
+            uint32_t w0[8], w1[8];
+            if (w.phase != PH_S) load_block_row(epi, r, c0, w0);
+            if (w.phase == PH_X) load_block_row(epi + kOperandBytes, r, c0, w1);
+            if (!split) {
+              uint32_t acc_v[16];
+              ptx::tmem_ld_32x16(taddr + (uint32_t)(g * 64 + c0), acc_v);
+              ptx::tmem_ld_wait_regs(acc_v);
 #pragma unroll
-          for (int q = 0; q < 16; ++q) split_pair(v[2 * q], v[2 * q + 1], w0[q], w1[q]);
-          store_chunk(p.arena + m.x[p.cur ^ 1] * 128 + x_at, w0);
-          store_chunk(p.arena + m.xlo * 128 + x_at, w1);
-        } else if (grow < m.m) {
-          const float scale = m.out_scale / m.sx;
-          unsigned short* out = reinterpret_cast<unsigned short*>(m.out);
-          const int gcol = j * kTile + c0;
-          if (m.tall) {
-#pragma unroll
-            for (int q = 0; q < 32; ++q)
-              if (gcol + q < m.n) out[(long long)(gcol + q) * m.m + grow] = out_bits(v[q] * scale, p.out_dt);
-          } else {
-            unsigned short* o = out + (long long)grow * m.n + gcol;
-            if ((m.n & 7) == 0 && gcol + 32 <= m.n) {
-#pragma unroll
-              for (int q = 0; q < 32; q += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-                  w[h] = out_bits(v[q + 2 * h] * scale, p.out_dt) | ((uint32_t)out_bits(v[q + 2 * h + 1] * scale, p.out_dt) << 16);
-                *reinterpret_cast<uint4*>(o + q) = make_uint4(w[0], w[1], w[2], w[3]);
-              }
+              for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(acc_v[q]);
             } else {
 #pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (gcol + q < m.n) o[q] = out_bits(v[q] * scale, p.out_dt);
+              for (int q = 0; q < 16; ++q) v[q] = 0.0f;
+              const float* src = part + r + (g * 64 + c0) * kTile;
+              int k = 0;
+              for (; k + 2 < m.splits; k += 3, src += 3 * (kTile * kN)) {   // three slices' loads in flight
+                float u[3][16];
+#pragma unroll
+                for (int q = 0; q < 48; ++q) u[q >> 4][q & 15] = __ldcg(src + (q >> 4) * (kTile * kN) + (q & 15) * kTile);
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] = ((v[q] + u[0][q]) + u[1][q]) + u[2][q];
+              }
+              for (; k < m.splits; ++k, src += kTile * kN) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] += __ldcg(src + q * kTile);
+              }
+            }
+            // this thread's 16 columns in block (ri, cb): 32 bytes
+            const long long sym_at = (s_block(m, ri, cb) + r) * 128 + c0 * 2;
+            const long long x_at = (x_block(m, ri, cb) + r) * 128 + c0 * 2;
+            if (w.phase == PH_S) {
+#pragma unroll
+              for (int q = 0; q < 16; ++q) v[q] *= s_scale;
+            } else if (w.phase == PH_B) {
+              const float kb = p.b * (kScaleB / kScaleS), kc = p.c * (kScaleB / (kScaleS * kScaleS));
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float2 s = unpack_half2(w0[q]);
+                v[2 * q] = fmaf(kc, v[2 * q], kb * s.x);
+                v[2 * q + 1] = fmaf(kc, v[2 * q + 1], kb * s.y);
+              }
+              const int dq = grow - (cb * 64 + c0);
+              if ((unsigned)dq < 16u) {   // the diagonal stays f32
+                float d = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                  d = q == dq ? v[q] : d;
+                  v[q] = q == dq ? 0.0f : v[q];
+                }
+                p.diag[m.diag + grow] = d * (1.0f / kScaleB);
+              }
+            } else {
+              const unsigned long long dg2 = ptx::f2_pack(dg, dg), one2 = ptx::f2_pack(1.0f, 1.0f), inv2 = ptx::f2_pack(1.0f / kScaleB, 1.0f / kScaleB);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float2 h = unpack_half2(w0[q]), l = unpack_half2(w1[q]);
+                const unsigned long long x = ptx::f2_fma(ptx::f2_pack(h.x, h.y), one2, ptx::f2_pack(l.x, l.y));
+                ptx::f2_unpack(ptx::f2_fma(dg2, x, ptx::f2_mul(ptx::f2_pack(v[2 * q], v[2 * q + 1]), inv2)), v[2 * q], v[2 * q + 1]);
+              }
+            }
+            if (w.phase != PH_X) {
+              uint8_t* dst = p.arena + (w.phase == PH_S ? m.s : m.b) * 128;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) w0[q] = pack_half2(v[2 * q], v[2 * q + 1]);
+              ptx::st_global_256(dst + sym_at, w0);
+              if (w.i != w.j) {   // the mirrored tile: lanes are neighbouring columns of it
+                unsigned short* mir = reinterpret_cast<unsigned short*>(dst + (s_block(m, cb >> 1, 2 * ri + (r >> 6)) + (cb & 1) * 64 + c0) * 128) + (r & 63);
+#pragma unroll
+                for (int q = 0; q < 16; ++q) mir[q * 64] = (unsigned short)(w0[q >> 1] >> (16 * (q & 1)));
+              }
+            } else if (!last) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) split_pair(v[2 * q], v[2 * q + 1], w0[q], w1[q]);
+              ptx::st_global_256(p.arena + m.x[cur ^ 1] * 128 + x_at, w0);
+              ptx::st_global_256(p.arena + m.xlo * 128 + x_at, w1);
+            } else {
+              unsigned short* out = reinterpret_cast<unsigned short*>(m.out);
+              const int gcol = cb * 64 + c0;
+              if (m.tall) {
+                if (grow < m.m)
+#pragma unroll
+                  for (int q = 0; q < 16; ++q)
+                    if (gcol + q < m.n) out[(long long)(gcol + q) * m.m + grow] = out_bits(v[q] * o_scale, p.out_dt);
+              } else if ((m.n & 7) == 0) {
+                if (grow < m.m)
+#pragma unroll
+                  for (int q = 0; q < 16; q += 8) {
+                    uint32_t pk[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                      pk[h] = out_bits(v[q + 2 * h] * o_scale, p.out_dt) | ((uint32_t)out_bits(v[q + 2 * h + 1] * o_scale, p.out_dt) << 16);
+                    if (gcol + q < m.n) *reinterpret_cast<uint4*>(out + (long long)grow * m.n + gcol + q) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                  }
+              } else {
+                // rows that do not start on a vector: through shared memory, so that lanes write neighbouring columns
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 16; ++q) sh.stage[warp - 4][lane][q] = out_bits(v[q] * o_scale, p.out_dt);
+                __syncwarp();
+#pragma unroll 4
+                for (int rr = lane >> 4; rr < 32; rr += 2) {
+                  const int orow = ri * kTile + quadrant * 32 + rr, c = lane & 15;
+                  if (orow < m.m && gcol + c < m.n) out[(long long)orow * m.n + gcol + c] = sh.stage[warp - 4][rr][c];
+                }
+              }
             }
           }
+          if (w.phase != PH_S) {   // the eight warps of this stage have read it
+            ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);
+            if ((tid & 255) == 0) ptx::mbar_arrive(bar(sh.empty[stage]));
+          }
+        }
+        if (!split) release();
+        // the tile is whole: its stores come before the count that lets others read it
+        ptx::named_barrier_sync(1, kEpiThreads);
+        if (tid == 0) {
+          __threadfence();
+          atomicAdd(&p.sync->done[w.mat][w.phase], 1u);
         }
       }
+      first_stage = (first_stage + w.k_blocks + (w.phase == PH_S ? 0 : kGroups)) % kStages;
+      __syncwarp();
+      if (lane == 0) arrive_lead(sh.item_empty[slot]);
     }
   }
   ptx::tcgen05_fence_before();
   __syncthreads();
+  if (PAIR) ptx::cluster_sync();   // the peer may still be signalling this CTA's barriers or reading its memory
   if (warp == 1) {
     ptx::tcgen05_fence_after();
-    ptx::tmem_dealloc(tmem, kTile);
+    if (PAIR) ptx::tmem_dealloc_2cta(tmem, 2 * kN);
+    else ptx::tmem_dealloc(tmem, 2 * kN);
   }
 }
 
@@ -491,9 +874,10 @@ int32_t encode_arena(CUtensorMap* map, void* arena, long long rows, int box_rows
 struct MuonPlan : he_plan {
   struct Round {
     int first;                 // first matrix of the list
+    bool pair;                 // CTA pairs on 256 x 256 tiles
     MuonTable table;           // pointers are filled in at launch
-    int sum_ctas, sym_ctas, x_ctas, pack_ctas;
-    size_t off_parts, off_diag, off_arena;
+    int sum_ctas, pack_ctas, iter_ctas, sync_words;
+    size_t off_sync, off_parts, off_diag, off_partial, off_arena;
     long long arena_rows;
   };
   std::vector<Round> rounds;
@@ -539,14 +923,25 @@ int32_t MuonPlan::check_overlap(const void* const* in, void* const* out) const {
   return HE_OK;
 }
 
-template <int PH> int32_t launch_gemm(const CUtensorMap& m128, const CUtensorMap& m64, const GemmArgs& a, int ctas, cudaStream_t stream) {
+template <bool PAIR>
+int32_t launch_iterate(const CUtensorMap& m128, const CUtensorMap& m64, const IterArgs& a, int ctas, cudaStream_t stream) {
+  auto kernel = muon_iterate_kernel<PAIR>;
   static bool configured = false;   // benign race: the attribute call is idempotent
   if (!configured) {
-    HE_CUDA(cudaFuncSetAttribute(muon_gemm_kernel<PH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem));
+    HE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kIterSmem));
     configured = true;
   }
-  muon_gemm_kernel<PH><<<ctas, kGemmThreads, kGemmSmem, stream>>>(m128, m64, a);
-  HE_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)ctas, 1, 1);
+  lc.blockDim = dim3(kGemmThreads, 1, 1);
+  lc.dynamicSmemBytes = kIterSmem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = PAIR ? 2 : 1; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  HE_CUDA(cudaLaunchKernelEx(&lc, kernel, m128, m64, a));
   return HE_OK;
 }
 
@@ -575,22 +970,18 @@ int32_t MuonPlan::launch(const void* const* in, void* const* out, void* ws, cuda
     CUtensorMap m128, m64;
     HE_TRY(encode_arena(&m128, arena, r.arena_rows, 128));
     HE_TRY(encode_arena(&m64, arena, r.arena_rows, 64));
-    muon_average_kernel<<<r.sum_ctas, kSumThreads, 0, stream>>>(t, st, table, parts);
+    MuonSync* sync = (MuonSync*)(w + r.off_sync);
+    muon_average_kernel<<<r.sum_ctas, kSumThreads, 0, stream>>>(t, st, table, parts, (unsigned*)sync, r.sync_words);
     HE_CUDA(cudaGetLastError());
-    muon_pack_kernel<<<r.pack_ctas, 256, 0, stream>>>(table, st, parts, arena);
+    muon_pack_kernel<<<r.pack_ctas, 256, 0, stream>>>(t, st, parts, arena);
     HE_CUDA(cudaGetLastError());
-    GemmArgs a{};
-    a.table = table; a.arena = arena; a.diag = (float*)(w + r.off_diag);
+    IterArgs a{};
+    a.table = table; a.sync = sync; a.arrive = (unsigned*)(sync + 1);
+    a.arena = arena; a.diag = (float*)(w + r.off_diag); a.partial = (float*)(w + r.off_partial);
     a.status = ctx->d_status; a.wait_limit_us = wait_limit_us; a.withhold_loads = withhold;
-    a.a = st.a; a.b = st.b; a.c = st.c; a.out_dt = st.out_dt;
-    for (int s = 0; s < steps; ++s) {
-      a.cur = s & 1;
-      a.last = s == steps - 1;
-      HE_TRY(launch_gemm<PH_S>(m128, m64, a, r.sym_ctas, stream));
-      HE_TRY(launch_gemm<PH_B>(m128, m64, a, r.sym_ctas, stream));
-      HE_TRY(launch_gemm<PH_X>(m128, m64, a, r.x_ctas, stream));
-    }
-    last_launches += 2 + 3 * steps;
+    a.steps = steps; a.a = st.a; a.b = st.b; a.c = st.c; a.out_dt = st.out_dt;
+    HE_TRY(r.pair ? launch_iterate<true>(m128, m64, a, r.iter_ctas, stream) : launch_iterate<false>(m128, m64, a, r.iter_ctas, stream));
+    last_launches += 3;
   }
   return HE_OK;
 } catch (const std::exception& e) {
@@ -627,17 +1018,46 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     MuonPlan::Round r{};
     r.first = first;
     r.table.count = std::min(kMaxMats, prm->count - first);
-    long long rows = 0, diag = 0, sym = 0, xt = 0, pack = 0, parts = 0;
+    const int sms = ctx_sm_count(ctx);
+    // Which tiles: a phase lasts as long as its deepest tile and a fixed part (waits, first loads, epilogue), or as its
+    // whole work spread over the workers, if that is longer.  Measured on a B200: 0.35 us a 64-deep block and 5 us fixed for
+    // 128 x 128 tiles, 0.41 us and 8 us for 256 x 256 tiles of a pair.  (A 1024 x 1024 matrix takes 166 us on single CTAs and
+    // 222 us on pairs, 2048 x 8192 851 and 767, 4096 x 4096 1790 and 1257.)
+    long long s_blocks1 = 0, s_blocks2 = 0;
     for (int i = 0; i < r.table.count; ++i) {
-      MuonMat& m = r.table.mat[i];
       const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
       if (h <= 0 || w <= 0) HE_FAIL(HE_ERR_INVALID, "muon: matrix %d is empty", first + i);
       if (std::min(h, w) > 32768 || std::max(h, w) > (1 << 20)) HE_FAIL(HE_ERR_UNSUPPORTED, "muon: matrix %d is larger than 32768 x 1048576", first + i);
+    }
+    auto step_us = [&](long long tile, int workers, double block_us, double fixed_us, long long* s_blocks) {
+      double work_s = 0, work_b = 0, work_x = 0, deep = 0;
+      for (int i = 0; i < r.table.count; ++i) {
+        const long long h = prm->rows[first + i], w = prm->cols[first + i], mm = std::min(h, w), nn = std::max(h, w);
+        const long long km = (mm + 63) / 64, kn = (nn + 63) / 64, ti = (mm + tile - 1) / tile, tj = (nn + tile - 1) / tile, sym = ti * (ti + 1) / 2;
+        work_s += (double)sym * kn;
+        work_b += (double)sym * km;
+        work_x += (double)ti * tj * km;
+        deep = std::max(deep, (double)km);
+      }
+      *s_blocks = (long long)work_s;
+      // S's sums are split where tiles are few
+      return block_us * (std::max(work_s / workers, std::min(deep, 16.0)) + std::max(work_b / workers, deep) + std::max(work_x / workers, deep)) + 3 * fixed_us;
+    };
+    r.pair = step_us(256, sms / 2, 0.41, 8.0, &s_blocks2) < step_us(128, sms, 0.35, 5.0, &s_blocks1);
+    const int unit = r.pair ? 2 : 1;
+    // S is split along n until a step's list of S items keeps every CTA (pair) busy, at 16 or more blocks of 64 columns a slice
+    // (a slice costs the write and the read of its f32 tile; 512 x 4608: 8 blocks 223 us, 16 198 us, 24 205 us)
+    const long long s_blocks = r.pair ? s_blocks2 : s_blocks1, workers = sms / unit;
+    const long long slice = std::max<long long>(16, (s_blocks + workers - 1) / workers);
+    long long rows = 0, diag = 0, items_s = 0, items_b = 0, items_x = 0, pack = 0, parts = 0, arrive = 0, partial = 0;
+    for (int i = 0; i < r.table.count; ++i) {
+      MuonMat& m = r.table.mat[i];
+      const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
       m.tall = h > w;
       m.m = (int)std::min(h, w);
       m.n = (int)std::max(h, w);
-      m.mt = (m.m + 127) / 128;
-      m.nt = (m.n + 127) / 128;
+      m.mt = (m.m + 128 * unit - 1) / (128 * unit) * unit;
+      m.nt = (m.n + 128 * unit - 1) / (128 * unit) * unit;
       m.out_scale = prm->scales ? prm->scales[first + i] : 1.0f;
       if (!std::isfinite(m.out_scale)) HE_FAIL(HE_ERR_INVALID, "muon: scale of matrix %d is not finite", first + i);
       const double side = std::sqrt((double)m.m * m.n);
@@ -649,9 +1069,17 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
       m.s = rows; rows += srows;
       m.b = rows; rows += srows;
       m.diag = diag; diag += (long long)m.mt * 128;
-      m.sym0 = (int)sym; sym += (long long)m.mt * (m.mt + 1) / 2;
-      m.x0 = (int)xt; xt += (long long)m.mt * m.nt;
-      m.pack0 = (int)pack; pack += (long long)m.mt * 2 * 2 * m.nt;
+      const long long ti = m.mt / unit, tj = m.nt / unit, tiles = ti * (ti + 1) / 2, blocks = (m.n + 63) / 64;
+      m.splits = (int)std::min<long long>(16, (blocks + slice - 1) / slice);
+      m.split_blocks = (int)((blocks + m.splits - 1) / m.splits);
+      m.splits = (int)((blocks + m.split_blocks - 1) / m.split_blocks);
+      m.arrive0 = (int)arrive; arrive += tiles * unit;
+      m.partial = partial;
+      if (m.splits > 1) partial += tiles * unit * m.splits * kTile * kTile * unit;
+      m.s0 = (int)items_s; items_s += tiles * m.splits;
+      m.b0 = (int)items_b; items_b += tiles;
+      m.x0 = (int)items_x; items_x += ti * tj;
+      m.pack0 = (int)pack; pack += (long long)m.mt * 2 * m.nt;
       // partial sums: CTAs of at least 4096 elements, at most 512 of them
       const long long total = (long long)m.m * m.n;
       long long chunks = std::min<long long>(512, (total + 4095) / 4096);
@@ -661,12 +1089,24 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
       m.part0 = (int)parts; parts += m.chunks;
       if (rows >= (1ll << 31) || pack >= (1ll << 31)) HE_FAIL(HE_ERR_UNSUPPORTED, "muon: the matrices of a plan exceed 2^31 workspace rows");
     }
-    r.sum_ctas = (int)parts; r.sym_ctas = (int)sym; r.x_ctas = (int)xt; r.pack_ctas = (int)pack;
+    if ((items_s + items_b + items_x) * (prm->steps + 1) + 4096 >= (1ll << 31)) HE_FAIL(HE_ERR_UNSUPPORTED, "muon: 2^31 or more work items");
+    for (int i = 0; i < r.table.count; ++i) {   // one list: S, then B, then X
+      r.table.mat[i].b0 += (int)items_s;
+      r.table.mat[i].x0 += (int)(items_s + items_b);
+    }
+    r.table.items_s = (int)items_s;
+    r.table.items_b = (int)(items_s + items_b);
+    r.table.items = (int)(items_s + items_b + items_x);
+    r.sum_ctas = (int)parts; r.pack_ctas = (int)pack;
+    r.iter_ctas = unit * (int)std::min<long long>(workers, std::max(items_s, items_x));
+    r.sync_words = (int)(sizeof(MuonSync) / 4 + arrive);
     r.arena_rows = rows;
     auto align = [](size_t v) { return (v + 1023) / 1024 * 1024; };
-    r.off_parts = align(sizeof(MuonTable));
+    r.off_sync = align(sizeof(MuonTable));
+    r.off_parts = align(r.off_sync + (size_t)r.sync_words * 4);
     r.off_diag = align(r.off_parts + (size_t)parts * sizeof(double));
-    r.off_arena = align(r.off_diag + (size_t)diag * sizeof(float));
+    r.off_partial = align(r.off_diag + (size_t)diag * sizeof(float));
+    r.off_arena = align(r.off_partial + (size_t)partial * sizeof(float));
     plan->workspace_bytes = std::max(plan->workspace_bytes, r.off_arena + (size_t)rows * 128);
     plan->rounds.push_back(r);
   }
