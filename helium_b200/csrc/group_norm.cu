@@ -1292,6 +1292,7 @@ __global__ void __launch_bounds__(512, 1) gn_backward_slab_kernel(const void* __
   if (b.size > 1) cluster_wait();
 }
 
+constexpr int kMaxSmem = 232448 - 1024;   // dynamic shared memory a CTA may ask for (with room for what kernels declare)
 // Bytes of shared memory of a slab CTA.
 size_t slab_smem(int direction, int dt, int values, int threads, int per, int cols, int groups, int channels) {
   const size_t tile = (size_t)per * cols * 16, lanes = (size_t)threads / cols;
@@ -1340,11 +1341,13 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
     lc.attrs = &attr;
     lc.numAttrs = 1;
     const int values = fold_values(V, g.f, g.cpg);
+    static SmemLimit limits[2][3];
+    SmemLimit& limit = limits[direction][!R && values == 1 ? 0 : !R && values == 2 ? 1 : 2];
     if (direction == HE_GN_FORWARD) {
       auto kernel = gn_forward_slab_kernel<DT, ACT, V, R>;
       if (!R && values == 1) kernel = gn_forward_slab_kernel<DT, ACT, 1, false>;
       if (!R && values == 2) kernel = gn_forward_slab_kernel<DT, ACT, 2, false>;
-      HE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      HE_TRY(limit.raise(kernel, ctx->device, kMaxSmem));
       HE_CUDA(cudaLaunchKernelEx(&lc, kernel, in[0], out[0], (const float*)in[1], (const float*)in[2], (float*)out[1], (float*)out[2], g));
       last_launches = 1;
       return HE_OK;
@@ -1352,7 +1355,7 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
     auto kernel = gn_backward_slab_kernel<DT, ACT, V, R>;
     if (!R && values == 1) kernel = gn_backward_slab_kernel<DT, ACT, 1, false>;
     if (!R && values == 2) kernel = gn_backward_slab_kernel<DT, ACT, 2, false>;
-    HE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    HE_TRY(limit.raise(kernel, ctx->device, kMaxSmem));
     HE_CUDA(cudaLaunchKernelEx(&lc, kernel, in[0], in[1], out[0], (const float*)in[2], (const float*)in[3], (const float*)in[4],
                                (const float*)in[5], (float*)ws, g));
     gn_param_grads_kernel<<<(2 * g.C + 31) / 32, dim3(32, 32), 0, st>>>((const float*)ws, (float*)out[1], (float*)out[2], g.N, g.C);
@@ -1481,7 +1484,7 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
         if (cs > 1 && per * (cs - 1) >= srows) continue;   // a CTA of the cluster would be left without rows
         if (per * cols * 16 > 232448) continue;
         const size_t sm = slab_smem(direction, prm->dtype, fold_values(V, g.f, g.cpg), threads, (int)per, cols, g.G / nblk, ch);
-        if (sm > 232448 - 1024) continue;
+        if (sm > kMaxSmem) continue;
         const int resident = std::max(1, std::min((int)(233472 / (sm + 1024)), (fwd ? 1024 : 512) / threads));
         const double ctas = (double)g.N * nblk * cs;
         const double vectors = std::ceil((double)per / (threads / cols));

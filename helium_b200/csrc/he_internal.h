@@ -1,6 +1,7 @@
 // Internal declarations shared by the translation units of libhelium_b200.so.
 #pragma once
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -120,6 +121,22 @@ class DeviceGuard {
  private:
   int prev_ = -1;
   bool switched_ = false, failed_ = false;
+};
+
+// Raises a kernel's limit of dynamic shared memory to all that an SM has, once on each device (the attribute belongs to
+// the function on the current device; a launch's own size decides occupancy).  One static object per kernel.
+class SmemLimit {
+ public:
+  template <class Kernel> int32_t raise(Kernel kernel, int device, int bytes) {
+    const uint64_t bit = device < 64 ? 1ull << device : 0ull;
+    if (bit && (done_.load(std::memory_order_relaxed) & bit)) return HE_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) HE_FAIL(HE_ERR_CUDA, "shared memory limit of a kernel: %s", cudaGetErrorString(e));
+    done_.fetch_or(bit, std::memory_order_relaxed);
+    return HE_OK;
+  }
+ private:
+  std::atomic<uint64_t> done_{0};
 };
 
 // NVTX range for the scope of a library call (visible in Nsight Systems / Compute timelines; the reference marks

@@ -160,6 +160,29 @@ __global__ void __launch_bounds__(kSumThreads) muon_average_kernel(const __grid_
   }
 }
 
+// 4 elements from e on (e a multiple of 4, tensors start on 16 bytes); those at or behind `total` are not read
+__device__ __forceinline__ void load_grad4(const void* g, int dt, long long e, long long total, float (&v)[4], bool read_only = true) {
+  if (e + 4 <= total) {
+    if (dt == HE_F32) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g) + e);
+      const float4 a = read_only ? __ldg(p) : *p;
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    } else {
+      const uint2 a = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const unsigned short*>(g) + e));
+      const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[2 * i] = dt == HE_BF16 ? bf16_bits_to_f32(w[i] & 0xffffu) : f16_bits_to_f32(w[i] & 0xffffu);
+        v[2 * i + 1] = dt == HE_BF16 ? bf16_bits_to_f32(w[i] >> 16) : f16_bits_to_f32(w[i] >> 16);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = e + i >= total ? 0.0f : dt == HE_F32 && !read_only ? reinterpret_cast<const float*>(g)[e + i] : load_grad(g, dt, e + i);
+  }
+}
+
 // hi + lo of two neighbouring values as two packed words
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -272,10 +295,11 @@ __global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ 
 // 128 rows and half of the column operand: half the bytes from L2 for the same products, which is what bounds 128 x 128
 // tiles (350 ns for the 32 KB of a 64-deep block, 13.5 TB/s over the chip, where the products take 140 ns).
 //
-// Warps: 0 items and loads, 1 products, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128 columns.  The tiles
-// that the epilogue reads (S, or X's two halves) follow a tile's operands through the same ring of stages, 64 columns a stage.
-// (Epilogue reads straight from L2, 64 bytes a lane, took 6 us a 128 x 128 tile; two teams on tiles that TMA brought took 3.5
-// us, their few warps waiting for their own arithmetic.)
+// Warps: 0 items and loads, 1 products, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128 columns.  Behind a
+// tile's operands the same ring hands the epilogue one stage for every 64 columns: TMA brings what it reads there (S, or X's
+// two halves), the results replace it in place and TMA takes them out, the mirrored tile of a symmetric product too.
+// (A thread owns a row.  Its own 32-byte loads and stores touch a line of its own each: 6 us a 128 x 128 tile with both, 3.2 us
+// with TMA loads and the stores as they were.)
 enum Phase { PH_S = 0, PH_B = 1, PH_X = 2 };
 constexpr int kTile = 128, kKBlock = 64;
 constexpr int kStages = 6;
@@ -294,7 +318,6 @@ struct IterShared {
   uint32_t tmem;
   int abort_flag;
   int last_split;
-  unsigned short stage[kEpiThreads / 32][32][18];   // a warp's 32 x 16 outputs
 };
 constexpr int kOffShared = kStages * 2 * kOperandBytes;
 constexpr int kIterSmem = kOffShared + (int)sizeof(IterShared) + 1024;
@@ -322,6 +345,11 @@ __device__ __forceinline__ void load_block_row(const uint8_t* block, int r, int 
     const uint4 v = *reinterpret_cast<const uint4*>(block + r * 128 + ((((c0 >> 3) + h) ^ (r & 7)) << 4));
     w[4 * h] = v.x; w[4 * h + 1] = v.y; w[4 * h + 2] = v.z; w[4 * h + 3] = v.w;
   }
+}
+__device__ __forceinline__ void store_block_row(uint8_t* block, int r, int c0, const uint32_t (&w)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    *reinterpret_cast<uint4*>(block + r * 128 + ((((c0 >> 3) + h) ^ (r & 7)) << 4)) = make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -404,6 +432,36 @@ template <bool PAIR> __device__ __forceinline__ Item decode_item(const MuonTable
   w.j = q - w.i * (w.i + 1) / 2;
   return w;
 }
+
+// 128 rows x 64 columns of the finished update from shared memory (128-byte swizzle) by 256 threads, lanes along the rows.
+__device__ __forceinline__ void copy_update(const MuonMat& m, const uint8_t* block, int row0, int col0, int tid) {
+  unsigned short* out = reinterpret_cast<unsigned short*>(m.out);
+  if ((m.n & 7) == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 3) + 32 * i, q = tid & 7;
+      if (row0 + r < m.m && col0 + 8 * q < m.n)
+        *reinterpret_cast<uint4*>(out + (long long)(row0 + r) * m.n + col0 + 8 * q) = *reinterpret_cast<const uint4*>(block + r * 128 + ((q ^ (r & 7)) << 4));
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      const int r = (tid >> 6) + 4 * i, c = tid & 63;
+      if (row0 + r < m.m && col0 + c < m.n)
+        out[(long long)(row0 + r) * m.n + col0 + c] = *reinterpret_cast<const unsigned short*>(block + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2);
+    }
+  }
+}
+
+// TMA store of a box of the arena from this CTA's shared memory
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int row) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row),
+               "r"(0), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }   // the source may be reused
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }             // the writes are made
 
 // store to the same place of CTA `rank`'s shared memory
 __device__ __forceinline__ void store_peer(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
@@ -555,16 +613,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
             row_b += kBlockRows;
           });
         }
-        if (w.phase == PH_S || !alive) continue;
-        // the epilogue's tiles, each CTA its own rows
+        if (!alive) break;
+        // the epilogue's stages, each CTA its own rows (S: room only)
         int row = (w.phase == PH_X ? xcur + ri * x_pitch : (int)m.s + ri * s_pitch) + kGroups * w.j * kBlockRows;
         const int lo = (int)m.xlo - xcur;
         for (int g = 0; g < kGroups; ++g, row += kBlockRows) {
           if (!ptx::mbar_wait(bar_empty(stage), phase ^ 1u, abort_flag, status, 2, stage, wait_us)) { alive = false; break; }
           const uint32_t dst = base + stage * 2 * kOperandBytes, eb = bar(sh.epi_full[slot][g]);
-          ptx::mbar_arrive_expect_tx(eb, (w.phase == PH_X ? 2 : 1) * kOperandBytes);
-          ptx::tma_load_3d(dst, &map128, eb, 0, row, 0);
-          if (w.phase == PH_X) ptx::tma_load_3d(dst + kOperandBytes, &map128, eb, 0, row + lo, 0);
+          if (w.phase == PH_S) {
+            ptx::mbar_arrive(eb);
+          } else {
+            ptx::mbar_arrive_expect_tx(eb, (w.phase == PH_X ? 2 : 1) * kOperandBytes);
+            ptx::tma_load_3d(dst, &map128, eb, 0, row, 0);
+            if (w.phase == PH_X) ptx::tma_load_3d(dst + kOperandBytes, &map128, eb, 0, row + lo, 0);
+          }
           epi_filled ^= 1u << (4 * slot + g);
           epi_any |= 1u << (4 * slot + g);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -622,7 +684,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
           }
           if (++stage == kStages) stage = 0;
         }
-        if (phase != PH_S) stage = (stage + kGroups) % kStages;   // the epilogue's tiles
+        stage = (stage + kGroups) % kStages;   // the epilogue's
         if (alive) {
           if (PAIR) {
             ptx::umma_commit_2cta(bar(sh.acc_full[acc]));
@@ -651,14 +713,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
       bool ok = ptx::mbar_wait(bar(sh.item_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, p.status, 3, slot, 2 * p.wait_limit_us);
       if (PAIR) fence_cluster_acquire();
       const Item w = sh.item[slot];
+      // What depends on the item alone is worked out while its products run.
+      const MuonMat& m = t.mat[ok && w.phase >= 0 ? w.mat : 0];
       const int ri = PAIR ? 2 * w.i + (int)rank : w.i;   // block row of this CTA
-      const int grow = ri * kTile + r;
-      float dg = 0.0f;         // of this row, while the products run
-      if (ok && w.phase == PH_X) dg = p.a + __ldcg(p.diag + t.mat[w.mat].diag + grow);
+      const int grow = ri * kTile + r, cb0 = kGroups * w.j;
+      const bool last = w.step == p.steps - 1;
+      const bool split = w.phase == PH_S && m.splits > 1;
+      const float s_scale = kScaleS / (m.sx * m.sx), o_scale = m.out_scale / m.sx;
+      float dg = 0.0f;         // B's diagonal at this row
+      int out_row, lo_row = 0, mir_row = 0;    // rows of the arena: of the tile's first block, of its low half, of the mirrored tile
+      const bool mirror = w.phase != PH_X && w.i != w.j;
+      if (w.phase == PH_X) {
+        if (ok) dg = p.a + __ldcg(p.diag + m.diag + grow);
+        const int at = (int)x_block(m, ri, cb0);
+        out_row = (int)m.x[(w.step & 1) ^ 1] + at;
+        lo_row = (int)m.xlo + at;
+      } else {
+        const int into = (int)(w.phase == PH_S ? m.s : m.b);
+        out_row = into + (int)s_block(m, ri, cb0);
+        mir_row = into + (int)s_block(m, cb0 >> 1, 2 * ri);
+      }
+      const int mir_pitch = 2 * m.mt * kBlockRows;   // from one block row to the next
+      float* part = nullptr;   // split tiles: slices side by side, each [column / 4][row][4]
+      if (split) part = p.partial + m.partial + (size_t)((w.i * (w.i + 1) / 2 + w.j) * kCtas + (int)rank) * m.splits * (kTile * kN) + r * 4;
       if (ok && w.phase >= 0) ok = ptx::mbar_wait(bar(sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u, abort_flag, p.status, 6, acc, p.wait_limit_us);
       if (!barrier_all(1, kEpiThreads, ok && w.phase >= 0)) break;
       ptx::tcgen05_fence_after();
-      const MuonMat& m = t.mat[w.mat];
       const uint32_t taddr = tmem + ((uint32_t)(quadrant * 32) << 16) + (uint32_t)(acc * kN);
       auto release = [&]() {   // the accumulator
         ptx::tcgen05_fence_before();
@@ -666,102 +746,107 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
         if (lane == 0) arrive_lead(sh.acc_empty[acc]);
       };
       bool finish = true;      // this CTA completes the tile
-      const bool split = w.phase == PH_S && m.splits > 1;
-      float* part = nullptr;
       if (split) {
-        // slices side by side, each [column][row]
-        const int tile = (w.i * (w.i + 1) / 2 + w.j) * kCtas + (int)rank;
-        part = p.partial + m.partial + (size_t)tile * m.splits * (kTile * kN);
-        float* mine = part + (size_t)w.split * (kTile * kN) + r;
+        float* mine = part + (size_t)w.split * (kTile * kN);
 #pragma unroll 1
         for (int c0 = team * 32; c0 < kN; c0 += 128) {
           uint32_t v[32];
           ptx::tmem_ld_32x32(taddr + (uint32_t)c0, v);
           ptx::tmem_ld_wait_regs(v);
 #pragma unroll
-          for (int q = 0; q < 32; ++q) mine[(c0 + q) * kTile] = __uint_as_float(v[q]);
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<uint4*>(mine + (size_t)(c0 / 4 + q) * (4 * kTile)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         }
         release();
         ptx::named_barrier_sync(1, kEpiThreads);
         if (tid == 0) {
           __threadfence();
-          const unsigned before = atomicAdd(p.arrive + m.arrive0 + tile, 1u);
+          const unsigned before = atomicAdd(p.arrive + m.arrive0 + (w.i * (w.i + 1) / 2 + w.j) * kCtas + (int)rank, 1u);
           sh.last_split = (before + 1) % (unsigned)m.splits == 0;
           __threadfence();
         }
         ptx::named_barrier_sync(1, kEpiThreads);
         finish = sh.last_split != 0;
       }
-      if (finish) {
-        const bool last = w.step == p.steps - 1;
-        const int cur = w.step & 1;
-        const float s_scale = kScaleS / (m.sx * m.sx), o_scale = m.out_scale / m.sx;
+      const int c0 = (team & 1) * 32;           // this team's columns of a 64-column block
 #pragma unroll 1
-        for (int g = buf; g < kGroups; g += 2) {
-          const int cb = kGroups * w.j + g;       // 64-column block of the matrix
-          const int stage = (first_stage + w.k_blocks + g) % kStages;
-          const uint8_t* const epi = smem + stage * 2 * kOperandBytes;
-          if (w.phase != PH_S) {
-            // (a wait that runs out leaves stale values behind, and the abort flag: the item loop ends at its next wait)
-            const int k = 4 * slot + g;
-            ptx::mbar_wait(bar(sh.epi_full[slot][g]), epi_parity >> k & 1u, abort_flag, p.status, 12, k, p.wait_limit_us);
-            epi_parity ^= 1u << k;
-            __syncwarp();
-          }
-#pragma unroll 1
-          for (int c0 = (team & 1) * 32, half = 0; half < 2; ++half, c0 += 16) {
-            float v[16];
-            uint32_t w0[8], w1[8];
-            if (w.phase != PH_S) load_block_row(epi, r, c0, w0);
-            if (w.phase == PH_X) load_block_row(epi + kOperandBytes, r, c0, w1);
-            if (!split) {
-              uint32_t acc_v[16];
-              ptx::tmem_ld_32x16(taddr + (uint32_t)(g * 64 + c0), acc_v);
-              ptx::tmem_ld_wait_regs(acc_v);
+      for (int g = buf; g < kGroups; g += 2) {
+        const int stage = (first_stage + w.k_blocks + g) % kStages;
+        uint8_t* const epi = smem + stage * 2 * kOperandBytes;    // in: S, or X's high half; out: the result's
+        uint8_t* const epi2 = epi + kOperandBytes;                // in: X's low half; out: that of the result, or the mirrored tile
+        uint32_t acc_v[32];
+        if (!split) ptx::tmem_ld_32x32(taddr + (uint32_t)(g * 64 + c0), acc_v);
+        {
+          // (a wait that runs out leaves stale values behind, and the abort flag: the item loop ends at its next wait)
+          const int k = 4 * slot + g;
+          ptx::mbar_wait(bar(sh.epi_full[slot][g]), epi_parity >> k & 1u, abort_flag, p.status, 12, k, p.wait_limit_us);
+          epi_parity ^= 1u << k;
+          __syncwarp();
+        }
+        if (finish) {
+          if (split) {
+            const float* src = part + (size_t)((g * 64 + c0) / 4) * (4 * kTile);
 #pragma unroll
-              for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(acc_v[q]);
-            } else {
+            for (int q = 0; q < 32; ++q) acc_v[q] = 0u;
+            for (int k = 0; k < m.splits; ++k, src += kTile * kN) {
+              float4 u[8];
 #pragma unroll
-              for (int q = 0; q < 16; ++q) v[q] = 0.0f;
-              const float* src = part + r + (g * 64 + c0) * kTile;
-              int k = 0;
-              for (; k + 2 < m.splits; k += 3, src += 3 * (kTile * kN)) {   // three slices' loads in flight
-                float u[3][16];
-#pragma unroll
-                for (int q = 0; q < 48; ++q) u[q >> 4][q & 15] = __ldcg(src + (q >> 4) * (kTile * kN) + (q & 15) * kTile);
-#pragma unroll
-                for (int q = 0; q < 16; ++q) v[q] = ((v[q] + u[0][q]) + u[1][q]) + u[2][q];
-              }
-              for (; k < m.splits; ++k, src += kTile * kN) {
-#pragma unroll
-                for (int q = 0; q < 16; ++q) v[q] += __ldcg(src + q * kTile);
-              }
-            }
-            // this thread's 16 columns in block (ri, cb): 32 bytes
-            const long long sym_at = (s_block(m, ri, cb) + r) * 128 + c0 * 2;
-            const long long x_at = (x_block(m, ri, cb) + r) * 128 + c0 * 2;
-            if (w.phase == PH_S) {
-#pragma unroll
-              for (int q = 0; q < 16; ++q) v[q] *= s_scale;
-            } else if (w.phase == PH_B) {
-              const float kb = p.b * (kScaleB / kScaleS), kc = p.c * (kScaleB / (kScaleS * kScaleS));
+              for (int q = 0; q < 8; ++q) u[q] = __ldcg(reinterpret_cast<const float4*>(src + q * (4 * kTile)));
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
-                const float2 s = unpack_half2(w0[q]);
-                v[2 * q] = fmaf(kc, v[2 * q], kb * s.x);
-                v[2 * q + 1] = fmaf(kc, v[2 * q + 1], kb * s.y);
+                acc_v[4 * q] = __float_as_uint(__uint_as_float(acc_v[4 * q]) + u[q].x);
+                acc_v[4 * q + 1] = __float_as_uint(__uint_as_float(acc_v[4 * q + 1]) + u[q].y);
+                acc_v[4 * q + 2] = __float_as_uint(__uint_as_float(acc_v[4 * q + 2]) + u[q].z);
+                acc_v[4 * q + 3] = __float_as_uint(__uint_as_float(acc_v[4 * q + 3]) + u[q].w);
               }
-              const int dq = grow - (cb * 64 + c0);
-              if ((unsigned)dq < 16u) {   // the diagonal stays f32
-                float d = 0.0f;
+            }
+          } else {
+            ptx::tmem_ld_wait_regs(acc_v);
+          }
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                  d = q == dq ? v[q] : d;
-                  v[q] = q == dq ? 0.0f : v[q];
+          for (int half = 0; half < 2; ++half) {
+            const int c = c0 + 16 * half;
+            float v[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(acc_v[16 * half + q]);
+            uint32_t w0[8], w1[8];
+            if (w.phase != PH_X) {
+              if (w.phase == PH_S) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] *= s_scale;
+              } else {
+                load_block_row(epi, r, c, w0);
+                const float kb = p.b * (kScaleB / kScaleS), kc = p.c * (kScaleB / (kScaleS * kScaleS));
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                  const float2 s = unpack_half2(w0[q]);
+                  v[2 * q] = fmaf(kc, v[2 * q], kb * s.x);
+                  v[2 * q + 1] = fmaf(kc, v[2 * q + 1], kb * s.y);
                 }
-                p.diag[m.diag + grow] = d * (1.0f / kScaleB);
+                const int dq = grow - ((cb0 + g) * 64 + c);
+                if ((unsigned)dq < 16u) {   // the diagonal stays f32
+                  float d = 0.0f;
+#pragma unroll
+                  for (int q = 0; q < 16; ++q) {
+                    d = q == dq ? v[q] : d;
+                    v[q] = q == dq ? 0.0f : v[q];
+                  }
+                  p.diag[m.diag + grow] = d * (1.0f / kScaleB);
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 8; ++q) w0[q] = pack_half2(v[2 * q], v[2 * q + 1]);
+              store_block_row(epi, r, c, w0);
+              if (mirror) {   // two pieces of 64 x 64, by the half of the rows; lanes are neighbouring columns of them
+                uint8_t* const to = epi2 + (r >> 6) * (kOperandBytes / 2) + (r & 7) * 2;
+                const int chunk = (r & 63) >> 3;
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                  *reinterpret_cast<unsigned short*>(to + (c + q) * 128 + ((chunk ^ (q & 7)) << 4)) = (unsigned short)(w0[q >> 1] >> (16 * (q & 1)));
               }
             } else {
+              load_block_row(epi, r, c, w0);
+              load_block_row(epi2, r, c, w1);
               const unsigned long long dg2 = ptx::f2_pack(dg, dg), one2 = ptx::f2_pack(1.0f, 1.0f), inv2 = ptx::f2_pack(1.0f / kScaleB, 1.0f / kScaleB);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
@@ -769,60 +854,49 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
                 const unsigned long long x = ptx::f2_fma(ptx::f2_pack(h.x, h.y), one2, ptx::f2_pack(l.x, l.y));
                 ptx::f2_unpack(ptx::f2_fma(dg2, x, ptx::f2_mul(ptx::f2_pack(v[2 * q], v[2 * q + 1]), inv2)), v[2 * q], v[2 * q + 1]);
               }
-            }
-            if (w.phase != PH_X) {
-              uint8_t* dst = p.arena + (w.phase == PH_S ? m.s : m.b) * 128;
+              if (!last) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) w0[q] = pack_half2(v[2 * q], v[2 * q + 1]);
-              ptx::st_global_256(dst + sym_at, w0);
-              if (w.i != w.j) {   // the mirrored tile: lanes are neighbouring columns of it
-                unsigned short* mir = reinterpret_cast<unsigned short*>(dst + (s_block(m, cb >> 1, 2 * ri + (r >> 6)) + (cb & 1) * 64 + c0) * 128) + (r & 63);
+                for (int q = 0; q < 8; ++q) split_pair(v[2 * q], v[2 * q + 1], w0[q], w1[q]);
+                store_block_row(epi, r, c, w0);
+                store_block_row(epi2, r, c, w1);
+              } else if (!m.tall) {
 #pragma unroll
-                for (int q = 0; q < 16; ++q) mir[q * 64] = (unsigned short)(w0[q >> 1] >> (16 * (q & 1)));
-              }
-            } else if (!last) {
+                for (int q = 0; q < 8; ++q) w0[q] = out_bits(v[2 * q] * o_scale, p.out_dt) | ((uint32_t)out_bits(v[2 * q + 1] * o_scale, p.out_dt) << 16);
+                store_block_row(epi, r, c, w0);
+              } else if (grow < m.m) {   // lanes are neighbouring columns of the tall update
+                unsigned short* out = reinterpret_cast<unsigned short*>(m.out) + grow;
+                const int gcol = (cb0 + g) * 64 + c;
 #pragma unroll
-              for (int q = 0; q < 8; ++q) split_pair(v[2 * q], v[2 * q + 1], w0[q], w1[q]);
-              ptx::st_global_256(p.arena + m.x[cur ^ 1] * 128 + x_at, w0);
-              ptx::st_global_256(p.arena + m.xlo * 128 + x_at, w1);
-            } else {
-              unsigned short* out = reinterpret_cast<unsigned short*>(m.out);
-              const int gcol = cb * 64 + c0;
-              if (m.tall) {
-                if (grow < m.m)
-#pragma unroll
-                  for (int q = 0; q < 16; ++q)
-                    if (gcol + q < m.n) out[(long long)(gcol + q) * m.m + grow] = out_bits(v[q] * o_scale, p.out_dt);
-              } else if ((m.n & 7) == 0) {
-                if (grow < m.m)
-#pragma unroll
-                  for (int q = 0; q < 16; q += 8) {
-                    uint32_t pk[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                      pk[h] = out_bits(v[q + 2 * h] * o_scale, p.out_dt) | ((uint32_t)out_bits(v[q + 2 * h + 1] * o_scale, p.out_dt) << 16);
-                    if (gcol + q < m.n) *reinterpret_cast<uint4*>(out + (long long)grow * m.n + gcol + q) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                  }
-              } else {
-                // rows that do not start on a vector: through shared memory, so that lanes write neighbouring columns
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 16; ++q) sh.stage[warp - 4][lane][q] = out_bits(v[q] * o_scale, p.out_dt);
-                __syncwarp();
-#pragma unroll 4
-                for (int rr = lane >> 4; rr < 32; rr += 2) {
-                  const int orow = ri * kTile + quadrant * 32 + rr, c = lane & 15;
-                  if (orow < m.m && gcol + c < m.n) out[(long long)orow * m.n + gcol + c] = sh.stage[warp - 4][rr][c];
-                }
+                for (int q = 0; q < 16; ++q)
+                  if (gcol + q < m.n) out[(long long)(gcol + q) * m.m] = (unsigned short)out_bits(v[q] * o_scale, p.out_dt);
               }
             }
           }
-          if (w.phase != PH_S) {   // the eight warps of this stage have read it
-            ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);
-            if ((tid & 255) == 0) ptx::mbar_arrive(bar(sh.empty[stage]));
-          }
+          ptx::fence_proxy_async_smem();
         }
+        ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);   // the block is whole
+        if (finish && w.phase == PH_X && last) {
+          if (!m.tall) {
+            copy_update(m, epi, ri * kTile, (cb0 + g) * 64, tid & 255);
+            ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);
+          }
+        } else if (finish && (tid & 255) == 0) {
+          const uint32_t src = base + stage * 2 * kOperandBytes;
+          tma_store_3d(&map128, src, out_row + g * kBlockRows);
+          if (w.phase == PH_X) tma_store_3d(&map128, src + kOperandBytes, lo_row + g * kBlockRows);
+          if (mirror) {
+            const int row = mir_row + (g >> 1) * mir_pitch + (g & 1) * 64;
+            tma_store_3d(&map64, src + kOperandBytes, row);
+            tma_store_3d(&map64, src + kOperandBytes + kOperandBytes / 2, row + kBlockRows);
+          }
+          tma_store_commit();
+          tma_store_wait_read();
+        }
+        if ((tid & 255) == 0) ptx::mbar_arrive(bar(sh.empty[stage]));
+      }
+      if (finish) {
         if (!split) release();
+        if ((tid & 255) == 0) tma_store_wait();
         // the tile is whole: its stores come before the count that lets others read it
         ptx::named_barrier_sync(1, kEpiThreads);
         if (tid == 0) {
@@ -830,7 +904,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
           atomicAdd(&p.sync->done[w.mat][w.phase], 1u);
         }
       }
-      first_stage = (first_stage + w.k_blocks + (w.phase == PH_S ? 0 : kGroups)) % kStages;
+      first_stage = (first_stage + w.k_blocks + kGroups) % kStages;
       __syncwarp();
       if (lane == 0) arrive_lead(sh.item_empty[slot]);
     }
@@ -842,6 +916,282 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
     ptx::tcgen05_fence_after();
     if (PAIR) ptx::tmem_dealloc_2cta(tmem, 2 * kN);
     else ptx::tmem_dealloc(tmem, 2 * kN);
+  }
+}
+
+// ---- small matrices: one CTA each, everything on chip ------------------------------------------------------------
+// Up to 128 x 320 the pair hi + lo of X (160 KB), S and B (32 KB each) stay in one SM's shared memory for the whole call:
+// average, norm, all steps and the update in one launch, with block barriers where the list of tiles has counters in memory
+// (5 us a phase there, 1.5 us here; a 64 x 288 filter takes 88 us by tiles).  The layout is the arena's: blocks of 128 rows x
+// 64 columns, 128-byte swizzle.  16 warps: thread = row, a warp's team 32 columns (of S, B) or 16 (of each block of X).
+constexpr int kSmallBlocks = 5, kSmallThreads = 512;
+struct SmallShared {
+  uint64_t done;
+  uint32_t tmem;
+  int abort_flag;
+  float diag[128];
+  double sums[kSmallThreads / 32];
+};
+constexpr int kOffSmallLo = kSmallBlocks * kOperandBytes, kOffSmallS = 2 * kOffSmallLo, kOffSmallB = kOffSmallS + 2 * kOperandBytes;
+constexpr int kOffSmallShared = kOffSmallB + 2 * kOperandBytes;
+constexpr int kSmallSmem = kOffSmallShared + (int)sizeof(SmallShared) + 1024;
+static_assert(kSmallSmem <= 232448, "shared memory budget of sm_100 exceeded");
+static_assert(128 * (64 * kSmallBlocks + 4) * 4 <= kOffSmallShared, "the f32 direction fits in front of the barriers");
+
+struct SmallArgs {
+  DeviceStatus* status;
+  unsigned wait_limit_us;
+  int withhold;
+  int steps;
+};
+
+__global__ void __launch_bounds__(kSmallThreads, 1) muon_small_kernel(const __grid_constant__ MuonTable t, const __grid_constant__ MuonStep st,
+                                                                      const __grid_constant__ SmallArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  SmallShared& sh = *reinterpret_cast<SmallShared*>(smem + kOffSmallShared);
+  const uint32_t base = ptx::smem_u32(smem), bar = ptx::smem_u32(&sh.done);
+  const MuonMat& m = t.mat[blockIdx.x];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int quadrant = warp & 3, team = warp >> 2, r = quadrant * 32 + lane;
+  const int blocks = (m.n + 63) / 64;
+  if (tid == 0) {
+    sh.abort_flag = 0;
+    ptx::mbar_init(bar, 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 0) {
+    ptx::tmem_alloc(ptx::smem_u32(&sh.tmem), 512);
+    ptx::tmem_relinquish();
+  }
+  // the average and the direction, as f32 [row][pitch] over the space of X, S and B
+  float* const d32 = reinterpret_cast<float*>(smem);
+  const int pitch = 64 * blocks + 4, total = m.m * m.n, inner = m.tall ? m.m : m.n;
+  for (int i = tid; i < 128 * pitch / 4; i += kSmallThreads) reinterpret_cast<float4*>(d32)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __syncthreads();
+  double sum = 0.0;
+  constexpr int U = 5;     // vectors of 4 elements a thread keeps in flight: one at a time, loading took 10 us of 49
+  for (int v0 = tid; v0 * 4 < total; v0 += U * kSmallThreads) {
+    float g[U][4], av[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_grad4(m.g, st.grad_dt, 4ll * (v0 + u * kSmallThreads), total, g[u]);
+    if (st.has_momentum)
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_grad4(m.avg, HE_F32, 4ll * (v0 + u * kSmallThreads), total, av[u], false);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e0 = 4 * (v0 + u * kSmallThreads);
+      int o = e0 / inner, i = e0 - o * inner;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (e0 + q < total) {
+          float d = g[u][q];
+          if (st.has_momentum) {
+            av[u][q] = fmaf(st.momentum, av[u][q], st.rest * d);
+            m.avg_out[e0 + q] = av[u][q];
+            d = direction(st, d, av[u][q]);
+          }
+          d32[m.tall ? i * pitch + o : o * pitch + i] = d;
+          sum = fma((double)d, (double)d, sum);
+        }
+        if (++i == inner) { i = 0; ++o; }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sh.sums[warp] = sum;
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  sum = 0.0;
+  for (int i = 0; i < kSmallThreads / 32; ++i) sum += sh.sums[i];
+  const float scale = (float)((double)m.sx / (sqrt(sum) + (double)st.eps));
+  // scaled and split into the blocks
+  {
+    float v[kSmallBlocks][16];
+#pragma unroll
+    for (int b = 0; b < kSmallBlocks; ++b)
+      if (b < blocks)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(d32 + r * pitch + b * 64 + team * 16 + 4 * q);
+          v[b][4 * q] = f.x; v[b][4 * q + 1] = f.y; v[b][4 * q + 2] = f.z; v[b][4 * q + 3] = f.w;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < kSmallBlocks; ++b)
+      if (b < blocks) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) split_pair(v[b][2 * q] * scale, v[b][2 * q + 1] * scale, hi[q], lo[q]);
+        store_block_row(smem + b * kOperandBytes, r, team * 16, hi);
+        store_block_row(smem + kOffSmallLo + b * kOperandBytes, r, team * 16, lo);
+      }
+  }
+  const float s_scale = kScaleS / (m.sx * m.sx), o_scale = m.out_scale / m.sx;
+  const float kb = st.b * (kScaleB / kScaleS), kc = st.c * (kScaleB / (kScaleS * kScaleS));
+  const uint32_t taddr = tmem + ((uint32_t)(quadrant * 32) << 16);
+  uint8_t* const s_tile = smem + kOffSmallS;
+  uint8_t* const b_tile = smem + kOffSmallB;
+  // Rows and columns behind the matrix are zeros from the start and stay so: their warps write S and B once.
+  const bool no_row = quadrant * 32 >= m.m, no_col = team * 32 >= m.m;
+  uint32_t parity = 0;
+  // Ends a phase's writes to shared memory and tensor memory reads, lets thread 0 issue the next products and waits for them.
+  auto products = [&](auto issue) {
+    ptx::fence_proxy_async_smem();
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    if (tid == 0 && !p.withhold) {
+      ptx::tcgen05_fence_after();
+      issue();
+      ptx::umma_commit(bar);
+    }
+    const bool ok = ptx::mbar_wait(bar, parity, &sh.abort_flag, p.status, 13, 0, p.wait_limit_us);
+    parity ^= 1u;
+    const bool all = __syncthreads_and(ok);
+    ptx::tcgen05_fence_after();
+    return all;
+  };
+  bool alive = true;
+  for (int step = 0; step < p.steps; ++step) {
+    // S = X X^T
+    alive = products([&] {
+      const uint32_t idesc = ptx::make_idesc_f16(0, 0, 0, 128, 128);
+      for (int b = 0; b < blocks; ++b) {
+        const uint64_t d = ptx::make_smem_desc_sw128(base + b * kOperandBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ptx::umma_f16(tmem, d + 2 * k, d + 2 * k, idesc, (b | k) != 0 ? 1u : 0u);
+      }
+    });
+    if (!alive) break;
+    if (step == 0 || !(no_row || no_col)) {
+      uint32_t a[32], w[8];
+      ptx::tmem_ld_32x32(taddr + team * 32, a);
+      ptx::tmem_ld_wait_regs(a);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = pack_half2(__uint_as_float(a[16 * h + 2 * q]) * s_scale, __uint_as_float(a[16 * h + 2 * q + 1]) * s_scale);
+        store_block_row(s_tile + (team >> 1) * kOperandBytes, r, (team & 1) * 32 + 16 * h, w);
+      }
+    }
+    // B = b S + c S^2, its diagonal apart
+    alive = products([&] {
+      const uint32_t idesc = ptx::make_idesc_f16(0, 0, 0, 128, 128);
+      for (int b = 0; b < 2; ++b) {
+        const uint64_t d = ptx::make_smem_desc_sw128(base + kOffSmallS + b * kOperandBytes, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ptx::umma_f16(tmem + 128, d + 2 * k, d + 2 * k, idesc, (b | k) != 0 ? 1u : 0u);
+      }
+    });
+    if (!alive) break;
+    if (step == 0 || !(no_row || no_col)) {
+      uint32_t a[32], w[8];
+      ptx::tmem_ld_32x32(taddr + 128 + team * 32, a);
+      ptx::tmem_ld_wait_regs(a);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[16];
+        load_block_row(s_tile + (team >> 1) * kOperandBytes, r, (team & 1) * 32 + 16 * h, w);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float2 s = unpack_half2(w[q]);
+          v[2 * q] = fmaf(kc, __uint_as_float(a[16 * h + 2 * q]), kb * s.x);
+          v[2 * q + 1] = fmaf(kc, __uint_as_float(a[16 * h + 2 * q + 1]), kb * s.y);
+        }
+        const int dq = r - (team * 32 + 16 * h);
+        if ((unsigned)dq < 16u) {
+          float d = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            d = q == dq ? v[q] : d;
+            v[q] = q == dq ? 0.0f : v[q];
+          }
+          sh.diag[r] = d * (1.0f / kScaleB);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) w[q] = pack_half2(v[2 * q], v[2 * q + 1]);
+        store_block_row(b_tile + (team >> 1) * kOperandBytes, r, (team & 1) * 32 + 16 * h, w);
+      }
+    }
+    // X <- a X + B X, in place
+    alive = products([&] {
+      // up to four blocks an instruction: the issuing thread spends some 65 cycles on each whatever its width
+      for (int b = 0; b < blocks; b += 4) {
+        const uint32_t idesc = ptx::make_idesc_f16(0, 0, 1, 128, 64 * min(4, blocks - b));
+        const uint64_t x = ptx::make_smem_desc_sw128(base + b * kOperandBytes, kOperandBytes, 1024);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t a = ptx::make_smem_desc_sw128(base + kOffSmallB + (k >> 2) * kOperandBytes, 16, 1024) + 2 * (k & 3);
+          ptx::umma_f16(tmem + b * 64, a, x + k * (2048 >> 4), idesc, k != 0 ? 1u : 0u);
+        }
+      }
+    });
+    if (!alive) break;
+    const float dg = st.a + sh.diag[r];
+    const bool last = step == p.steps - 1;
+    if (!no_row) {
+#pragma unroll
+      for (int b0 = 0; b0 < kSmallBlocks; b0 += 2) {   // two blocks' loads before the first one's arithmetic
+        if (b0 >= blocks) break;
+        uint32_t a[2][16], w0[2][8], w1[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (b0 + u < blocks) {
+            const uint8_t* const hi = smem + (b0 + u) * kOperandBytes;
+            ptx::tmem_ld_32x16(taddr + (b0 + u) * 64 + team * 16, a[u]);
+            load_block_row(hi, r, team * 16, w0[u]);
+            load_block_row(hi + kOffSmallLo, r, team * 16, w1[u]);
+          }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (b0 + u < blocks) {
+            uint8_t* const hi = smem + (b0 + u) * kOperandBytes;
+            ptx::tmem_ld_wait_regs(a[u]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float2 h = unpack_half2(w0[u][q]), l = unpack_half2(w1[u][q]);
+              const float x = fmaf(dg, h.x + l.x, __uint_as_float(a[u][2 * q]) * (1.0f / kScaleB));
+              const float y = fmaf(dg, h.y + l.y, __uint_as_float(a[u][2 * q + 1]) * (1.0f / kScaleB));
+              if (!last) split_pair(x, y, w0[u][q], w1[u][q]);
+              else w0[u][q] = out_bits(x * o_scale, st.out_dt) | ((uint32_t)out_bits(y * o_scale, st.out_dt) << 16);
+            }
+            store_block_row(hi, r, team * 16, w0[u]);
+            if (!last) store_block_row(hi + kOffSmallLo, r, team * 16, w1[u]);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  if (alive) {
+    unsigned short* out = reinterpret_cast<unsigned short*>(m.out);
+#pragma unroll 2
+    for (int v = tid; v * 4 < total; v += kSmallThreads) {
+      const int e0 = 4 * v;
+      int o = e0 / inner, i = e0 - o * inner;
+      uint32_t h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int row = m.tall ? i : o, c = m.tall ? o : i;
+        h[q] = e0 + q < total ? *reinterpret_cast<const unsigned short*>(smem + (c >> 6) * kOperandBytes + row * 128 +
+                                                                        ((((c & 63) >> 3) ^ (row & 7)) << 4) + (c & 7) * 2) : 0u;
+        if (++i == inner) { i = 0; ++o; }
+      }
+      if (e0 + 4 <= total) *reinterpret_cast<uint2*>(out + e0) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+      else
+        for (int q = 0; q < 4 && e0 + q < total; ++q) out[e0 + q] = (unsigned short)h[q];
+    }
+  } else if (tid == 0 && !p.withhold) {   // products in flight may not write tensor memory that is freed
+    int never = 0;
+    ptx::mbar_wait(bar, parity ^ 1u, &never, p.status, 8, 0, p.wait_limit_us);
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    ptx::tcgen05_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
   }
 }
 
@@ -874,6 +1224,7 @@ int32_t encode_arena(CUtensorMap* map, void* arena, long long rows, int box_rows
 struct MuonPlan : he_plan {
   struct Round {
     int first;                 // first matrix of the list
+    bool small;                // every matrix fits an SM: muon_small_kernel
     bool pair;                 // CTA pairs on 256 x 256 tiles
     MuonTable table;           // pointers are filled in at launch
     int sum_ctas, pack_ctas, iter_ctas, sync_words;
@@ -924,13 +1275,10 @@ int32_t MuonPlan::check_overlap(const void* const* in, void* const* out) const {
 }
 
 template <bool PAIR>
-int32_t launch_iterate(const CUtensorMap& m128, const CUtensorMap& m64, const IterArgs& a, int ctas, cudaStream_t stream) {
+int32_t launch_iterate(const CUtensorMap& m128, const CUtensorMap& m64, const IterArgs& a, int ctas, int device, cudaStream_t stream) {
   auto kernel = muon_iterate_kernel<PAIR>;
-  static bool configured = false;   // benign race: the attribute call is idempotent
-  if (!configured) {
-    HE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kIterSmem));
-    configured = true;
-  }
+  static SmemLimit limit;
+  HE_TRY(limit.raise(kernel, device, kIterSmem));
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)ctas, 1, 1);
   lc.blockDim = dim3(kGemmThreads, 1, 1);
@@ -963,6 +1311,15 @@ int32_t MuonPlan::launch(const void* const* in, void* const* out, void* ws, cuda
       m.avg = st.has_momentum ? (const float*)in[count + k] : nullptr;
       m.avg_out = st.has_momentum ? (float*)out[count + k] : nullptr;
     }
+    if (r.small) {
+      static SmemLimit limit;
+      HE_TRY(limit.raise(muon_small_kernel, ctx->device, kSmallSmem));
+      const SmallArgs sa{ctx->d_status, wait_limit_us, withhold, steps};
+      muon_small_kernel<<<t.count, kSmallThreads, kSmallSmem, stream>>>(t, st, sa);
+      HE_CUDA(cudaGetLastError());
+      last_launches += 1;
+      continue;
+    }
     uint8_t* w = (uint8_t*)ws;
     MuonTable* table = (MuonTable*)w;
     double* parts = (double*)(w + r.off_parts);
@@ -980,7 +1337,8 @@ int32_t MuonPlan::launch(const void* const* in, void* const* out, void* ws, cuda
     a.arena = arena; a.diag = (float*)(w + r.off_diag); a.partial = (float*)(w + r.off_partial);
     a.status = ctx->d_status; a.wait_limit_us = wait_limit_us; a.withhold_loads = withhold;
     a.steps = steps; a.a = st.a; a.b = st.b; a.c = st.c; a.out_dt = st.out_dt;
-    HE_TRY(r.pair ? launch_iterate<true>(m128, m64, a, r.iter_ctas, stream) : launch_iterate<false>(m128, m64, a, r.iter_ctas, stream));
+    HE_TRY(r.pair ? launch_iterate<true>(m128, m64, a, r.iter_ctas, ctx->device, stream)
+                  : launch_iterate<false>(m128, m64, a, r.iter_ctas, ctx->device, stream));
     last_launches += 3;
   }
   return HE_OK;
@@ -1019,6 +1377,12 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     r.first = first;
     r.table.count = std::min(kMaxMats, prm->count - first);
     const int sms = ctx_sm_count(ctx);
+    // Every matrix of this part of the list fits an SM (where only some do, the others' tiles leave room for theirs)
+    r.small = true;
+    for (int i = 0; i < r.table.count; ++i) {
+      const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
+      r.small = r.small && h > 0 && w > 0 && std::min(h, w) <= 128 && std::max(h, w) <= 64 * kSmallBlocks;
+    }
     // Which tiles: a phase lasts as long as its deepest tile and a fixed part (waits, first loads, epilogue), or as its
     // whole work spread over the workers, if that is longer.  Measured on a B200: 0.35 us a 64-deep block and 5 us fixed for
     // 128 x 128 tiles, 0.41 us and 8 us for 256 x 256 tiles of a pair.  (A 1024 x 1024 matrix takes 166 us on single CTAs and
@@ -1107,7 +1471,7 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     r.off_diag = align(r.off_parts + (size_t)parts * sizeof(double));
     r.off_partial = align(r.off_diag + (size_t)diag * sizeof(float));
     r.off_arena = align(r.off_partial + (size_t)partial * sizeof(float));
-    plan->workspace_bytes = std::max(plan->workspace_bytes, r.off_arena + (size_t)rows * 128);
+    if (!r.small) plan->workspace_bytes = std::max(plan->workspace_bytes, r.off_arena + (size_t)rows * 128);
     plan->rounds.push_back(r);
   }
   char desc[256];

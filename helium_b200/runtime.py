@@ -6,7 +6,6 @@ goes through `he_launch`; nothing here computes on the host.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import List, Optional, Sequence
 
@@ -17,7 +16,7 @@ from ._abi import HeConv2dFusion, HeConv2dParams, HeGroupNormParams, HeMuonParam
 from ._lib import HeliumError, check, lib
 
 _TORCH_DTYPES = None
-_NO_CONTEXT = contextlib.nullcontext()
+_DEVICES = {}
 
 
 def _torch():
@@ -28,6 +27,24 @@ def _torch():
         _TORCH_DTYPES = {ir.F16: torch.float16, ir.BF16: torch.bfloat16, ir.F32: torch.float32,
                          ir.U32: torch.int32, ir.BOOL: torch.int32}
     return torch
+
+
+def _cuda_device(torch, index: int):
+    d = _DEVICES.get(index)
+    if d is None:
+        d = _DEVICES[index] = torch.device("cuda", index)
+    return d
+
+
+def _checked_ptr(t, spec, dev: int, what: str, i: int) -> int:
+    """Address of a dense tensor of the shape and type that the plan wants there, on the plan's device."""
+    if t.shape != spec[0] or t.dtype is not spec[1]:
+        raise ValueError(f"{what} {i} must be {spec[1]} {spec[0]}, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what} {i} must be a contiguous CUDA tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"{what} {i} is on {t.device}, the plan on cuda:{dev}")
+    return t.data_ptr()
 
 
 def storage_elems(dtype: int, n: int) -> int:
@@ -84,7 +101,7 @@ class Plan:
         self.ctx = ctx
         self._workspace = None
         self._in_specs = None       # (shape, dtype) of every input, for the plans whose launches are checked
-        self._ws_bytes = None
+        self._torch_specs = None    # the same in torch's terms, with the outputs' and the workspace's size
 
     # -- constructors ------------------------------------------------------------------------------
     @staticmethod
@@ -235,11 +252,11 @@ class Plan:
         torch = _torch()
         if len(inputs) != self.n_inputs:
             raise ValueError(f"plan takes {self.n_inputs} inputs, got {len(inputs)}")
+        if self._in_specs is not None:
+            return self._launch_checked(torch, inputs, outputs, stream)
         for t in inputs:
             if not t.is_cuda or not t.is_contiguous():
                 raise ValueError("inputs must be contiguous CUDA tensors")
-        if self._in_specs is not None:
-            return self._launch_checked(torch, inputs, outputs, stream)
         if outputs is None:
             outputs = self.alloc_outputs(inputs[0].device if inputs else "cuda")
         ws = self.workspace_bytes
@@ -256,41 +273,46 @@ class Plan:
         of the plan's device, and the workspace belongs to this launch alone (taken from torch's allocator on the launching
         stream: part of the graph's pool under capture), so launches on several streams and several captured graphs never
         share one."""
-        dev = self.ctx.device if self.ctx else None
-
-        def checked(t, spec, what, i):
-            if tuple(t.shape) != spec[0] or t.dtype != _TORCH_DTYPES[spec[1]]:
-                raise ValueError(f"{what} {i} must be {_TORCH_DTYPES[spec[1]]} {spec[0]}, got {t.dtype} {tuple(t.shape)}")
-            if dev is not None and t.device.index != dev:
-                raise ValueError(f"{what} {i} is on {t.device}, the plan on cuda:{dev}")
-            return t.data_ptr()
-
-        ins = [checked(t, spec, "input", i) for i, (t, spec) in enumerate(zip(inputs, self._in_specs))]
-        current = torch.cuda.current_stream(dev)
-        if stream is None:
-            target = current
-        else:
+        if self._torch_specs is None:
+            as_torch = lambda spec: (tuple(spec[0]), _TORCH_DTYPES[spec[1]])  # noqa: E731
+            in_specs = [as_torch(spec) for spec in self._in_specs]
+            out_specs = [as_torch(spec) for spec in zip(self.out_shapes, self.out_dtypes)]
+            # an input of the same shape and type, or of the type: a new output is made like it (torch.empty's keywords
+            # cost more than a microsecond each time)
+            like = [in_specs.index(o) if o in in_specs else None for o in out_specs]
+            of_type = [next((k for k, i in enumerate(in_specs) if i[1] is o[1]), None) for o in out_specs]
+            self._torch_specs = (in_specs, out_specs, list(zip(like, of_type)), self.workspace_bytes,
+                                 C.c_void_p * len(in_specs), C.c_void_p * len(out_specs))
+        in_specs = self._torch_specs[0]
+        dev = self.ctx.device if self.ctx else 0
+        ins = [_checked_ptr(t, spec, dev, "input", i) for i, (t, spec) in enumerate(zip(inputs, in_specs))]
+        if stream is not None:
             target = torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream
-        with torch.cuda.stream(target) if target != current else _NO_CONTEXT:
-            if outputs is None:
-                dev_t = inputs[0].device
-                outputs = [torch.empty(shape, dtype=_TORCH_DTYPES[dt], device=dev_t) for shape, dt in zip(self.out_shapes, self.out_dtypes)]
-                outs = [t.data_ptr() for t in outputs]
-            else:
-                if len(outputs) != len(self.out_shapes):
-                    raise ValueError(f"plan writes {len(self.out_shapes)} outputs, got {len(outputs)}")
-                outs = []
-                for i, t in enumerate(outputs):
-                    if not t.is_cuda or not t.is_contiguous():
-                        raise ValueError("outputs must be contiguous CUDA tensors")
-                    outs.append(checked(t, (tuple(self.out_shapes[i]), self.out_dtypes[i]), "output", i))
-            if self._ws_bytes is None:
-                self._ws_bytes = self.workspace_bytes
-            wptr = 0
-            if self._ws_bytes:
-                ws = torch.empty(self._ws_bytes + 256, dtype=torch.uint8, device=inputs[0].device)
-                wptr = (ws.data_ptr() + 255) // 256 * 256
-            self.launch_ptrs(ins, outs, wptr, target)
+            with torch.cuda.stream(target):
+                return self._launch_on(torch, target.cuda_stream, dev, inputs, ins, outputs)
+        return self._launch_on(torch, torch.cuda.current_stream(dev).cuda_stream, dev, inputs, ins, outputs)
+
+    def _launch_on(self, torch, stream_ptr, dev, inputs, ins, outputs):
+        _, out_specs, sources, ws_bytes, in_array, out_array = self._torch_specs
+        if outputs is None:
+            outputs = []
+            for (like, of_type), (shape, dt) in zip(sources, out_specs):
+                if like is not None:
+                    outputs.append(torch.empty_like(inputs[like]))
+                elif of_type is not None:
+                    outputs.append(inputs[of_type].new_empty(shape))
+                else:
+                    outputs.append(torch.empty(shape, dtype=dt, device=_cuda_device(torch, dev)))
+            outs = [t.data_ptr() for t in outputs]
+        else:
+            if len(outputs) != len(out_specs):
+                raise ValueError(f"plan writes {len(out_specs)} outputs, got {len(outputs)}")
+            outs = [_checked_ptr(t, spec, dev, "output", i) for i, (t, spec) in enumerate(zip(outputs, out_specs))]
+        wptr = 0
+        if ws_bytes:
+            ws = torch.empty(ws_bytes + 256, dtype=torch.uint8, device=_cuda_device(torch, dev))
+            wptr = (ws.data_ptr() + 255) // 256 * 256
+        check(lib.he_launch(self._h, in_array(*ins), out_array(*outs), wptr, stream_ptr))
         return outputs
 
     def close(self) -> None:
