@@ -295,9 +295,12 @@ __global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ 
 // 128 rows and half of the column operand: half the bytes from L2 for the same products, which is what bounds 128 x 128
 // tiles (350 ns for the 32 KB of a 64-deep block, 13.5 TB/s over the chip, where the products take 140 ns).
 //
-// Warps: 0 items and loads, 1 products, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128 columns.  Behind a
+// Warps: 0 items and loads, 1 products, 2 and 3 stores, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128
+// columns.  Behind a
 // tile's operands the same ring hands the epilogue one stage for every 64 columns: TMA brings what it reads there (S, or X's
 // two halves), the results replace it in place and TMA takes them out, the mirrored tile of a symmetric product too.
+// What follows a store (its completion, the count) is the store warps' business: an epilogue that waited for them itself took
+// 5.8 us a tile of the conv net's X, whose products take 3.8.
 // (A thread owns a row.  Its own 32-byte loads and stores touch a line of its own each: 6 us a 128 x 128 tile with both, 3.2 us
 // with TMA loads and the stores as they were.)
 enum Phase { PH_S = 0, PH_B = 1, PH_X = 2 };
@@ -314,10 +317,11 @@ struct Item {
 struct IterShared {
   MuonTable table;
   Item item[kSlots];
-  uint64_t full[kStages], empty[kStages], item_full[kSlots], item_empty[kSlots], acc_full[2], acc_empty[2], epi_full[kSlots][4], drain;
+  uint64_t full[kStages], empty[kStages], item_full[kSlots], item_empty[kSlots], acc_full[2], acc_empty[2], epi_full[kSlots][4], written[kSlots][4], drain;
   uint32_t tmem;
   int abort_flag;
   int last_split;
+  int unfinished[kSlots][2];   // the item's tile waits for other slices; for either store warp
 };
 constexpr int kOffShared = kStages * 2 * kOperandBytes;
 constexpr int kIterSmem = kOffShared + (int)sizeof(IterShared) + 1024;
@@ -496,12 +500,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
   if (threadIdx.x == 0) {
     sh.abort_flag = 0;
     for (int s = 0; s < kStages; ++s) { ptx::mbar_init(bar(sh.full[s]), 1); ptx::mbar_init(bar(sh.empty[s]), 1); }
-    for (int s = 0; s < kSlots; ++s) { ptx::mbar_init(bar(sh.item_full[s]), 1); ptx::mbar_init(bar(sh.item_empty[s]), kCtas * (kEpiThreads / 32)); }
+    for (int s = 0; s < kSlots; ++s) { ptx::mbar_init(bar(sh.item_full[s]), 1); ptx::mbar_init(bar(sh.item_empty[s]), kCtas * (kEpiThreads / 32 + 2)); }
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(bar(sh.acc_full[s]), 1);
       ptx::mbar_init(bar(sh.acc_empty[s]), kCtas * (kEpiThreads / 32));
     }
-    for (int s = 0; s < kSlots * 4; ++s) ptx::mbar_init(bar(sh.epi_full[s >> 2][s & 3]), 1);
+    for (int s = 0; s < kSlots * 4; ++s) { ptx::mbar_init(bar(sh.epi_full[s >> 2][s & 3]), 1); ptx::mbar_init(bar(sh.written[s >> 2][s & 3]), 8); }
     ptx::mbar_init(bar(sh.drain), 1);
     ptx::fence_mbar_init();
   }
@@ -550,8 +554,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
           if (w.phase >= 0) {
             const MuonMat& m = t.mat[w.mat];
             const unsigned* done = p.sync->done[w.mat];
-            const unsigned ti = (unsigned)(PAIR ? m.mt >> 1 : m.mt), tj = (unsigned)(PAIR ? m.nt >> 1 : m.nt), sym = ti * (ti + 1) / 2 * kCtas;
-            if (w.phase == PH_S) alive = wait_count(done + PH_X, (unsigned)w.step * ti * tj * kCtas, abort_flag, p.status, p.wait_limit_us);
+            const unsigned ti = (unsigned)(PAIR ? m.mt >> 1 : m.mt), tj = (unsigned)(PAIR ? m.nt >> 1 : m.nt), sym = ti * (ti + 1) / 2 * (2 * kCtas);   // two store warps a CTA
+            if (w.phase == PH_S) alive = wait_count(done + PH_X, (unsigned)w.step * ti * tj * (2 * kCtas), abort_flag, p.status, p.wait_limit_us);
             else alive = wait_count(done + (w.phase == PH_B ? PH_S : PH_B), (unsigned)(w.step + 1) * sym, abort_flag, p.status, p.wait_limit_us);
             if (!alive) break;
           }
@@ -701,7 +705,63 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
         ptx::mbar_wait(bar(sh.drain), 0, &never, p.status, 8, 0, p.wait_limit_us);
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp < 4) {
+    // ===================== stores: warp 2 + buf, the 64-column blocks of its parity =====================
+    if (lane == 0) {
+      const int buf = warp - 2;
+      int first_stage = 0;
+      unsigned parity = 0;           // of the next use of each `written` barrier
+      for (int n = 0;; ++n) {
+        const int slot = n % kSlots;
+        if (!ptx::mbar_wait(bar(sh.item_full[slot]), (uint32_t)(n / kSlots) & 1u, abort_flag, p.status, 3, slot, 2 * p.wait_limit_us)) break;
+        if (PAIR) fence_cluster_acquire();
+        const Item w = sh.item[slot];
+        if (w.phase < 0) break;
+        const MuonMat& m = t.mat[w.mat];
+        const int ri = PAIR ? 2 * w.i + (int)rank : w.i, cb0 = kGroups * w.j;
+        const bool mirror = w.phase != PH_X && w.i != w.j, direct = w.phase == PH_X && w.step == p.steps - 1;
+        int out_row, lo_row = 0, mir_row = 0;    // rows of the arena: of the tile's first block, of its low half, of the mirrored tile
+        if (w.phase == PH_X) {
+          const int at = (int)x_block(m, ri, cb0);
+          out_row = (int)m.x[(w.step & 1) ^ 1] + at;
+          lo_row = (int)m.xlo + at;
+        } else {
+          const int into = (int)(w.phase == PH_S ? m.s : m.b);
+          out_row = into + (int)s_block(m, ri, cb0);
+          mir_row = into + (int)s_block(m, cb0 >> 1, 2 * ri);
+        }
+        const int mir_pitch = 2 * m.mt * kBlockRows;   // from one block row to the next
+        bool alive = true, finish = true;
+        for (int g = buf; g < kGroups; g += 2) {
+          const int k = 4 * slot + g, stage = (first_stage + w.k_blocks + g) % kStages;
+          if (!ptx::mbar_wait(bar(sh.written[slot][g]), parity >> k & 1u, abort_flag, p.status, 14, k, 2 * p.wait_limit_us)) { alive = false; break; }
+          parity ^= 1u << k;
+          finish = sh.unfinished[slot][buf] == 0;
+          if (finish && !direct) {
+            const uint32_t src = base + stage * 2 * kOperandBytes;
+            tma_store_3d(&map128, src, out_row + g * kBlockRows);
+            if (w.phase == PH_X) tma_store_3d(&map128, src + kOperandBytes, lo_row + g * kBlockRows);
+            if (mirror) {
+              const int row = mir_row + (g >> 1) * mir_pitch + (g & 1) * 64;
+              tma_store_3d(&map64, src + kOperandBytes, row);
+              tma_store_3d(&map64, src + kOperandBytes + kOperandBytes / 2, row + kBlockRows);
+            }
+            tma_store_commit();
+            tma_store_wait_read();
+          }
+          ptx::mbar_arrive(bar(sh.empty[stage]));
+        }
+        tma_store_wait();
+        if (!alive) break;
+        if (finish) {   // this half of the tile is in memory: only then does the count say so
+          __threadfence();
+          atomicAdd(&p.sync->done[w.mat][w.phase], 1u);
+        }
+        first_stage = (first_stage + w.k_blocks + kGroups) % kStages;
+        arrive_lead(sh.item_empty[slot]);
+      }
+    }
+  } else {
     // ===================== epilogue: thread = row of the tile, team = 32 columns of every 128 =====================
     const int quadrant = warp & 3, team = (warp - 4) >> 2, buf = team >> 1, r = quadrant * 32 + lane;
     const int tid = threadIdx.x - 128;
@@ -721,19 +781,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
       const bool split = w.phase == PH_S && m.splits > 1;
       const float s_scale = kScaleS / (m.sx * m.sx), o_scale = m.out_scale / m.sx;
       float dg = 0.0f;         // B's diagonal at this row
-      int out_row, lo_row = 0, mir_row = 0;    // rows of the arena: of the tile's first block, of its low half, of the mirrored tile
       const bool mirror = w.phase != PH_X && w.i != w.j;
-      if (w.phase == PH_X) {
-        if (ok) dg = p.a + __ldcg(p.diag + m.diag + grow);
-        const int at = (int)x_block(m, ri, cb0);
-        out_row = (int)m.x[(w.step & 1) ^ 1] + at;
-        lo_row = (int)m.xlo + at;
-      } else {
-        const int into = (int)(w.phase == PH_S ? m.s : m.b);
-        out_row = into + (int)s_block(m, ri, cb0);
-        mir_row = into + (int)s_block(m, cb0 >> 1, 2 * ri);
-      }
-      const int mir_pitch = 2 * m.mt * kBlockRows;   // from one block row to the next
+      if (ok && w.phase == PH_X) dg = p.a + __ldcg(p.diag + m.diag + grow);
       float* part = nullptr;   // split tiles: slices side by side, each [column / 4][row][4]
       if (split) part = p.partial + m.partial + (size_t)((w.i * (w.i + 1) / 2 + w.j) * kCtas + (int)rank) * m.splits * (kTile * kN) + r * 4;
       if (ok && w.phase >= 0) ok = ptx::mbar_wait(bar(sh.acc_full[acc]), (uint32_t)(n >> 1) & 1u, abort_flag, p.status, 6, acc, p.wait_limit_us);
@@ -768,6 +817,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
         ptx::named_barrier_sync(1, kEpiThreads);
         finish = sh.last_split != 0;
       }
+      if ((tid & 255) == 0) sh.unfinished[slot][buf] = finish ? 0 : 1;
       const int c0 = (team & 1) * 32;           // this team's columns of a 64-column block
 #pragma unroll 1
       for (int g = buf; g < kGroups; g += 2) {
@@ -873,37 +923,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) muon_iterate_kernel(const __g
             }
           }
           ptx::fence_proxy_async_smem();
-        }
-        ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);   // the block is whole
-        if (finish && w.phase == PH_X && last) {
-          if (!m.tall) {
+          if (w.phase == PH_X && last && !m.tall) {
+            ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);   // the block is whole
             copy_update(m, epi, ri * kTile, (cb0 + g) * 64, tid & 255);
-            ptx::named_barrier_sync(2 + buf, kEpiThreads / 2);
           }
-        } else if (finish && (tid & 255) == 0) {
-          const uint32_t src = base + stage * 2 * kOperandBytes;
-          tma_store_3d(&map128, src, out_row + g * kBlockRows);
-          if (w.phase == PH_X) tma_store_3d(&map128, src + kOperandBytes, lo_row + g * kBlockRows);
-          if (mirror) {
-            const int row = mir_row + (g >> 1) * mir_pitch + (g & 1) * 64;
-            tma_store_3d(&map64, src + kOperandBytes, row);
-            tma_store_3d(&map64, src + kOperandBytes + kOperandBytes / 2, row + kBlockRows);
-          }
-          tma_store_commit();
-          tma_store_wait_read();
         }
-        if ((tid & 255) == 0) ptx::mbar_arrive(bar(sh.empty[stage]));
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(sh.written[slot][g]));
       }
-      if (finish) {
-        if (!split) release();
-        if ((tid & 255) == 0) tma_store_wait();
-        // the tile is whole: its stores come before the count that lets others read it
-        ptx::named_barrier_sync(1, kEpiThreads);
-        if (tid == 0) {
-          __threadfence();
-          atomicAdd(&p.sync->done[w.mat][w.phase], 1u);
-        }
-      }
+      if (!split) release();
       first_stage = (first_stage + w.k_blocks + kGroups) % kStages;
       __syncwarp();
       if (lane == 0) arrive_lead(sh.item_empty[slot]);
@@ -1223,7 +1251,7 @@ int32_t encode_arena(CUtensorMap* map, void* arena, long long rows, int box_rows
 
 struct MuonPlan : he_plan {
   struct Round {
-    int first;                 // first matrix of the list
+    std::vector<int> index;    // the table's matrices in the caller's list
     bool small;                // every matrix fits an SM: muon_small_kernel
     bool pair;                 // CTA pairs on 256 x 256 tiles
     MuonTable table;           // pointers are filled in at launch
@@ -1255,7 +1283,7 @@ int32_t MuonPlan::check_overlap(const void* const* in, void* const* out) const {
   v.reserve(4 * count);
   for (const Round& r : rounds)
     for (int i = 0; i < r.table.count; ++i) {
-      const int k = r.first + i;
+      const int k = r.index[i];
       const uintptr_t n = (uintptr_t)r.table.mat[i].m * r.table.mat[i].n;
       auto add = [&](const void* p, uintptr_t bytes, bool w) { v.push_back({(uintptr_t)p, (uintptr_t)p + bytes, w}); };
       add(in[k], n * dtype_bytes(st.grad_dt), false);
@@ -1305,7 +1333,7 @@ int32_t MuonPlan::launch(const void* const* in, void* const* out, void* ws, cuda
     MuonTable t = r.table;   // a copy: the plan is not changed by a launch
     for (int i = 0; i < t.count; ++i) {
       MuonMat& m = t.mat[i];
-      const int k = r.first + i;
+      const int k = r.index[i];
       m.g = in[k];
       m.out = out[k];
       m.avg = st.has_momentum ? (const float*)in[count + k] : nullptr;
@@ -1372,15 +1400,21 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
   st.out_dt = prm->out_dtype;
   st.a = prm->coef[0]; st.b = prm->coef[1]; st.c = prm->coef[2];
   st.eps = prm->eps;
+  // Smallest products first: at every border of a phase the small matrices' items, whose own phase is over by then, come
+  // before those of the large ones, which have to wait (the conv net's filters: 297 us, largest first 322 us).
+  std::vector<int> order((size_t)prm->count);
+  for (int i = 0; i < prm->count; ++i) order[i] = i;
+  auto weight = [&](int i) { return (double)std::min(prm->rows[i], prm->cols[i]) * (double)prm->rows[i] * (double)prm->cols[i]; };
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return weight(a) < weight(b); });
   for (int first = 0; first < prm->count; first += kMaxMats) {
     MuonPlan::Round r{};
-    r.first = first;
     r.table.count = std::min(kMaxMats, prm->count - first);
+    r.index.assign(order.begin() + first, order.begin() + first + r.table.count);
     const int sms = ctx_sm_count(ctx);
     // Every matrix of this part of the list fits an SM (where only some do, the others' tiles leave room for theirs)
     r.small = true;
     for (int i = 0; i < r.table.count; ++i) {
-      const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
+      const int64_t h = prm->rows[r.index[i]], w = prm->cols[r.index[i]];
       r.small = r.small && h > 0 && w > 0 && std::min(h, w) <= 128 && std::max(h, w) <= 64 * kSmallBlocks;
     }
     // Which tiles: a phase lasts as long as its deepest tile and a fixed part (waits, first loads, epilogue), or as its
@@ -1389,14 +1423,14 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     // 222 us on pairs, 2048 x 8192 851 and 767, 4096 x 4096 1790 and 1257.)
     long long s_blocks1 = 0, s_blocks2 = 0;
     for (int i = 0; i < r.table.count; ++i) {
-      const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
-      if (h <= 0 || w <= 0) HE_FAIL(HE_ERR_INVALID, "muon: matrix %d is empty", first + i);
-      if (std::min(h, w) > 32768 || std::max(h, w) > (1 << 20)) HE_FAIL(HE_ERR_UNSUPPORTED, "muon: matrix %d is larger than 32768 x 1048576", first + i);
+      const int64_t h = prm->rows[r.index[i]], w = prm->cols[r.index[i]];
+      if (h <= 0 || w <= 0) HE_FAIL(HE_ERR_INVALID, "muon: matrix %d is empty", r.index[i]);
+      if (std::min(h, w) > 32768 || std::max(h, w) > (1 << 20)) HE_FAIL(HE_ERR_UNSUPPORTED, "muon: matrix %d is larger than 32768 x 1048576", r.index[i]);
     }
     auto step_us = [&](long long tile, int workers, double block_us, double fixed_us, long long* s_blocks) {
       double work_s = 0, work_b = 0, work_x = 0, deep = 0;
       for (int i = 0; i < r.table.count; ++i) {
-        const long long h = prm->rows[first + i], w = prm->cols[first + i], mm = std::min(h, w), nn = std::max(h, w);
+        const long long h = prm->rows[r.index[i]], w = prm->cols[r.index[i]], mm = std::min(h, w), nn = std::max(h, w);
         const long long km = (mm + 63) / 64, kn = (nn + 63) / 64, ti = (mm + tile - 1) / tile, tj = (nn + tile - 1) / tile, sym = ti * (ti + 1) / 2;
         work_s += (double)sym * kn;
         work_b += (double)sym * km;
@@ -1416,14 +1450,14 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     long long rows = 0, diag = 0, items_s = 0, items_b = 0, items_x = 0, pack = 0, parts = 0, arrive = 0, partial = 0;
     for (int i = 0; i < r.table.count; ++i) {
       MuonMat& m = r.table.mat[i];
-      const int64_t h = prm->rows[first + i], w = prm->cols[first + i];
+      const int64_t h = prm->rows[r.index[i]], w = prm->cols[r.index[i]];
       m.tall = h > w;
       m.m = (int)std::min(h, w);
       m.n = (int)std::max(h, w);
       m.mt = (m.m + 128 * unit - 1) / (128 * unit) * unit;
       m.nt = (m.n + 128 * unit - 1) / (128 * unit) * unit;
-      m.out_scale = prm->scales ? prm->scales[first + i] : 1.0f;
-      if (!std::isfinite(m.out_scale)) HE_FAIL(HE_ERR_INVALID, "muon: scale of matrix %d is not finite", first + i);
+      m.out_scale = prm->scales ? prm->scales[r.index[i]] : 1.0f;
+      if (!std::isfinite(m.out_scale)) HE_FAIL(HE_ERR_INVALID, "muon: scale of matrix %d is not finite", r.index[i]);
       const double side = std::sqrt((double)m.m * m.n);
       m.sx = (float)std::ldexp(1.0, std::min(15, (int)std::floor(std::log2(side))));
       const long long xrows = (long long)m.mt * 2 * m.nt * kBlockRows, srows = (long long)m.mt * 2 * m.mt * kBlockRows;
@@ -1472,7 +1506,7 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     r.off_partial = align(r.off_diag + (size_t)diag * sizeof(float));
     r.off_arena = align(r.off_partial + (size_t)partial * sizeof(float));
     if (!r.small) plan->workspace_bytes = std::max(plan->workspace_bytes, r.off_arena + (size_t)rows * 128);
-    plan->rounds.push_back(r);
+    plan->rounds.push_back(std::move(r));
   }
   char desc[256];
   snprintf(desc, sizeof desc, "muon: %d matri%s, %s gradients%s, %d Newton-Schulz steps on tcgen05 (f16 operands, hi + lo pair), %s updates", prm->count,
