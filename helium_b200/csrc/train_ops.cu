@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(256) sgd_momentum_kernel(float* __restrict__ w
     float gv;
     if (sizeof(G) == 4) gv = reinterpret_cast<const float*>(g)[i];
     else gv = bf16_bits_to_f32(reinterpret_cast<const unsigned short*>(g)[i]);
-    const float a = first ? gv : gv * (1.0f - m) + avg[i] * m;
+    const float a = first || !avg ? gv : gv * (1.0f - m) + avg[i] * m;   // no average: plain SGD
     if (avg) avg[i] = a;
     const float nw = w[i] - a * lr;
     w[i] = nw;
