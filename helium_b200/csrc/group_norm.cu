@@ -122,27 +122,43 @@ __device__ __forceinline__ f2 sigmoid2(f2 z) {
   un(mul2(z, pk(-1.4426950408889634f, -1.4426950408889634f)), a, b);
   return reciprocals(add2(pk(ex2(a), ex2(b)), pk(1.0f, 1.0f)));
 }
-// Normal cumulative distribution, and exp(-z^2 / 2) beside it.  f32 tensors take erfcf; for 16-bit ones Abramowitz &
-// Stegun 7.1.26 gives erfc(|x|) as a polynomial times exp(-x^2), used as such on the negative side (no cancellation in the
-// tail), absolute error 1.5e-7.  |x| is capped at 20, where erfc is 0 in f32.
+// Normal cumulative distribution, and exp(-z^2 / 2) beside it: half of erfc(|z| / sqrt 2) on the negative side (no
+// cancellation in the tail), one minus that on the other.  f32 tensors take the Chebyshev form of Numerical Recipes
+// ("erfcc": t exp(-x^2 + a polynomial in t), relative error 1.2e-7; erff and erfcf of the library took most of the kernel's time),
+// 16-bit ones Abramowitz & Stegun 7.1.26 (a polynomial in t times exp(-x^2), absolute error 1.5e-7).  |x| is capped at 20, where
+// erfc is 0 in f32.
 template <bool kExact> __device__ __forceinline__ f2 normal_cdf2(f2 z, f2& bell) {
   float za, zb;
   un(z, za, zb);
-  if (kExact) {
-    bell = pk(__expf(-0.5f * za * za), __expf(-0.5f * zb * zb));
-    return pk(0.5f * erfcf(za * -0.70710678118654752440f), 0.5f * erfcf(zb * -0.70710678118654752440f));
-  }
   const f2 ax = pk(fminf(fabsf(za) * 0.70710678118654752440f, 20.0f), fminf(fabsf(zb) * 0.70710678118654752440f, 20.0f));
-  const f2 t = reciprocals(fma2(ax, pk(0.3275911f, 0.3275911f), pk(1.0f, 1.0f)));
-  f2 poly = fma2(pk(1.061405429f, 1.061405429f), t, pk(-1.453152027f, -1.453152027f));
-  poly = fma2(poly, t, pk(1.421413741f, 1.421413741f));
-  poly = fma2(poly, t, pk(-0.284496736f, -0.284496736f));
-  poly = fma2(poly, t, pk(0.254829592f, 0.254829592f));
-  float ea, eb;
-  un(mul2(mul2(ax, ax), pk(-1.4426950408889634f, -1.4426950408889634f)), ea, eb);
+  auto c2 = [](float c) { return pk(c, c); };
+  const f2 log2e = c2(1.4426950408889634f), nsq = mul2(mul2(ax, ax), c2(-1.0f));
+  float ea, eb, ta, tb;
+  un(mul2(nsq, log2e), ea, eb);
   bell = pk(ex2(ea), ex2(eb));
-  float ta, tb;
-  un(mul2(mul2(poly, mul2(t, pk(0.5f, 0.5f))), bell), ta, tb);
+  f2 half;
+  if (kExact) {
+    const f2 t = reciprocals(fma2(ax, c2(0.5f), c2(1.0f)));
+    f2 p = fma2(c2(0.17087277f), t, c2(-0.82215223f));
+    p = fma2(p, t, c2(1.48851587f));
+    p = fma2(p, t, c2(-1.13520398f));
+    p = fma2(p, t, c2(0.27886807f));
+    p = fma2(p, t, c2(-0.18628806f));
+    p = fma2(p, t, c2(0.09678418f));
+    p = fma2(p, t, c2(0.37409196f));
+    p = fma2(p, t, c2(1.00002368f));
+    p = fma2(p, t, c2(-1.26551223f));
+    un(mul2(add2(nsq, p), log2e), ea, eb);
+    half = mul2(mul2(t, c2(0.5f)), pk(ex2(ea), ex2(eb)));
+  } else {
+    const f2 t = reciprocals(fma2(ax, c2(0.3275911f), c2(1.0f)));
+    f2 p = fma2(c2(1.061405429f), t, c2(-1.453152027f));
+    p = fma2(p, t, c2(1.421413741f));
+    p = fma2(p, t, c2(-0.284496736f));
+    p = fma2(p, t, c2(0.254829592f));
+    half = mul2(mul2(p, mul2(t, c2(0.5f))), bell);
+  }
+  un(half, ta, tb);
   return pk(za < 0.0f ? ta : 1.0f - ta, zb < 0.0f ? tb : 1.0f - tb);
 }
 // NaN stays NaN in each of them (fmaxf would turn a rectified NaN into 0).
@@ -469,14 +485,55 @@ template <int V> __device__ __forceinline__ void thread_channels(const GnGeom& g
   }
 }
 
+// 16 bytes from global to shared memory without passing through registers; a thread reads only what it copied itself
+__device__ __forceinline__ void copy16(const void* dst_shared, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst_shared)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits until at most `n` of the thread's latest groups are in flight
+__device__ __forceinline__ void copy_wait(int n) {
+  if (n >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+// Walks a thread's vectors of T tensors in order, `kDepth` of each in flight: copies into a ring of its own in shared
+// memory ([place][tensor][thread], so no two threads share any of it).  With two or four loads held in registers instead,
+// the passes over a [2,512,512,128] tensor ran at 3.1 and 3.8 TB/s.
+constexpr int kDepth = 8;
+template <int T, class F>
+__device__ __forceinline__ void stream_vectors(const uint4* (&src)[T], size_t step, int count, uint4* ring, F fn) {
+  uint4* const mine = ring + threadIdx.x;
+  const int place = T * blockDim.x;
+#pragma unroll
+  for (int i = 0; i < kDepth - 1; ++i) {
+    if (i < count)
+#pragma unroll
+      for (int t = 0; t < T; ++t) copy16(mine + i * place + t * blockDim.x, src[t] + i * step);
+    copy_commit();
+  }
+  for (int i = 0; i < count; ++i) {
+    if (i + kDepth - 1 < count)
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        copy16(mine + ((i + kDepth - 1) % kDepth) * place + t * blockDim.x, src[t] + (size_t)(i + kDepth - 1) * step);
+    copy_commit();
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    uint4 v[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) v[t] = mine[(i % kDepth) * place + t * blockDim.x];
+    fn(i, v);
+  }
+}
+
 // =================================================================================================
 // Tensors whose (picture, group) slabs are too large for on-chip memory: partial sums of slices, a fold, a second pass.
 // =================================================================================================
 // Moments of each column of a slice: part[n][slice][e] = (sum, sum of squares about the column's mean in the slice).
 template <int DT, bool kRagged>
-__global__ void __launch_bounds__(512) gn_moments_kernel(const void* __restrict__ x, float2* __restrict__ part, GnGeom g) {
-  constexpr int V = Elem<DT>::V, U = 4;
-  extern __shared__ float sh[];
+__global__ void __launch_bounds__(512, 1) gn_moments_kernel(const void* __restrict__ x, float2* __restrict__ part, GnGeom g) {
+  constexpr int V = Elem<DT>::V;
+  extern __shared__ float sh[];        // the ring, then (behind the barrier of the first fold's caller) the folds' space
   float* red = sh;
   float* tree = red + blockDim.x * V;
   float* col = tree + blockDim.x;      // [cols * V]
@@ -488,28 +545,52 @@ __global__ void __launch_bounds__(512) gn_moments_kernel(const void* __restrict_
   m.clear();
   if (lane < g.lanes && vcol * V < g.W) {
     const int pitch = g.W / V;
-    const uint4* src = reinterpret_cast<const uint4*>(x) + (h.f0 + lane) * pitch + vcol;
-    const int rows = (int)max(0ll, h.f1 - h.f0 - lane);
-    const size_t step = (size_t)g.lanes * pitch;
-    if (rows > 0) m.start(src[0]);
-    int r = 0;
-    for (; r + (U - 1) * g.lanes < rows; r += U * g.lanes, src += U * step) {
-      uint4 v[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) v[k] = src[k * step];
-#pragma unroll
-      for (int k = 0; k < U; ++k) m.add(v[k]);
-      m.inner += (float)U;
-    }
-    for (; r < rows; r += g.lanes, src += step) {
-      m.add(src[0]);
-      m.inner += 1.0f;
-    }
+    const uint4* src[1] = {reinterpret_cast<const uint4*>(x) + (h.f0 + lane) * pitch + vcol};
+    const int rows = (int)max(0ll, h.f1 - h.f0 - lane), count = (rows + g.lanes - 1) / g.lanes;
+    stream_vectors<1>(src, (size_t)g.lanes * pitch, count, reinterpret_cast<uint4*>(sh), [&](int i, const uint4 (&v)[1]) {
+      if (i == 0) m.start(v[0]);
+      m.add(v[0]);
+    });
+    m.inner = (float)count;
     if (kRagged)
       edge_rows(g, h, lane, [&](long long row) {
         const long long e = row * g.W + (long long)vcol * V;
         m.add_edge(load_edge<DT>(x, e, g.total), e, h.lo, h.hi);
       });
+  }
+  float t[V], mean[V];
+  m.sums(t);
+  __syncthreads();                     // every thread is through with its ring
+  column_sums<V>(g, t, j, lane, red, tree, col);
+  const int w = g.cols * V;
+  if (g.nblk == 1) {
+    // all columns are here: (sum, sum of squares about the slice's mean) of each group
+    float* grp = col + w;              // [G]
+    float2* out = part + ((size_t)n * gridDim.x + blockIdx.x) * (size_t)g.G;
+    const int ln = threadIdx.x & 31;
+    auto fold = [&](auto put) {
+      for (int k = threadIdx.x >> 5; k < g.G; k += blockDim.x >> 5) {
+        float s = 0.0f;
+        for (int r = 0; r < g.f; ++r)
+          for (int c = ln; c < g.cpg; c += 32) s += col[r * g.C + k * g.cpg + c];
+        s = warp_sum(s);
+        if (ln == 0) put(k, s);
+      }
+      __syncthreads();
+    };
+    const float count = share_rows(g, h) * g.cpg;
+    fold([&](int k, float s) {
+      out[k].x = s;
+      grp[k] = count > 0.0f ? s / count : 0.0f;
+    });
+    int c[V];
+    thread_channels<V>(g, lane < g.lanes ? j : 0, c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) mean[i] = grp[g.div_cpg.div((uint32_t)c[i])];
+    m.squares(mean, t);
+    column_sums<V>(g, t, j, lane, red, tree, col);
+    fold([&](int k, float s) { out[k].y = s; });
+    return;
   }
   // values of column e in this slice: rows of the picture whose place in the super-row is e / C
   auto column_count = [&](int e) -> float {
@@ -519,9 +600,6 @@ __global__ void __launch_bounds__(512) gn_moments_kernel(const void* __restrict_
     if (a >= b) return 0.0f;
     return (float)((b - k + g.f - 1) / g.f - (a - k + g.f - 1) / g.f);
   };
-  float t[V], mean[V];
-  m.sums(t);
-  column_sums<V>(g, t, j, lane, red, tree, col);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const float cc = lane < g.lanes ? column_count(j * V + i) : 0.0f;
@@ -529,7 +607,6 @@ __global__ void __launch_bounds__(512) gn_moments_kernel(const void* __restrict_
   }
   m.squares(mean, t);
   // the first fold's totals leave shared memory before the second one overwrites them
-  const int w = g.cols * V;
   float2* out = part + ((size_t)n * gridDim.x + blockIdx.x) * (size_t)(g.nblk * w) + (size_t)blk * w;
   for (int e = threadIdx.x; e < w; e += blockDim.x) out[e].x = col[e];
   __syncthreads();
@@ -537,36 +614,39 @@ __global__ void __launch_bounds__(512) gn_moments_kernel(const void* __restrict_
   for (int e = threadIdx.x; e < w; e += blockDim.x) out[e].y = col[e];
 }
 
-// mean and rstd of each (picture, group) from the slices' column moments; one CTA of 128 threads per (picture, group).
-__global__ void __launch_bounds__(128) gn_fold_moments_kernel(const float2* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
+// mean and rstd of each (picture, group) from the slices' moments, of the group (one item a slice) or, where a slice is cut
+// into column blocks, of its columns; one CTA of 256 threads per (picture, group).
+__global__ void __launch_bounds__(256) gn_fold_moments_kernel(const float2* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
                                                               GnGeom g, int slices, int pitch) {
-  __shared__ float sh[4];
+  __shared__ float sh[8];
   const int n = blockIdx.x / g.G, k = blockIdx.x % g.G;
-  const int per_slice = g.f * g.cpg, items = slices * per_slice;
+  const bool whole = g.nblk == 1;
+  const int per_slice = whole ? 1 : g.f * g.cpg, items = slices * per_slice;
   const long long row0 = (long long)n * g.P, row1 = row0 + g.P, first = row0 / g.f;
   auto block_sum = [&](float s) {
     s = warp_sum(s);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
     __syncthreads();
-    const float t = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    const float t = ((sh[0] + sh[1]) + (sh[2] + sh[3])) + ((sh[4] + sh[5]) + (sh[6] + sh[7]));
     __syncthreads();
     return t;
   };
   auto item = [&](int i, float& cnt) -> float2 {
-    const int sl = i / per_slice, r = i - sl * per_slice, kk = r / g.cpg, c = r - kk * g.cpg;
+    const int sl = whole ? i : i / per_slice, r = i - sl * per_slice, kk = whole ? 0 : r / g.cpg, c = r - kk * g.cpg;
     const long long s0 = first + (long long)sl * g.per, s1 = min((row1 + g.f - 1) / g.f, s0 + g.per);
     const long long a = max(s0 * g.f, row0), b = min(s1 * g.f, row1);
+    if (whole) {
+      cnt = (float)max(0ll, b - a) * g.cpg;
+      return part[((size_t)n * slices + sl) * g.G + k];
+    }
     cnt = a < b ? (float)((b - kk + g.f - 1) / g.f - (a - kk + g.f - 1) / g.f) : 0.0f;
     return part[((size_t)n * slices + sl) * pitch + (size_t)kk * g.C + (size_t)k * g.cpg + c];
   };
   float s = 0.0f, cnt;
-  for (int i = threadIdx.x; i < items; i += 128) {
-    const float2 v = item(i, cnt);
-    s += v.x;
-  }
+  for (int i = threadIdx.x; i < items; i += 256) s += item(i, cnt).x;
   const float m = block_sum(s) * g.inv_count;
   float q = 0.0f;
-  for (int i = threadIdx.x; i < items; i += 128) {
+  for (int i = threadIdx.x; i < items; i += 256) {
     const float2 v = item(i, cnt);
     if (cnt > 0.0f) {
       const float d = v.x / cnt - m;
@@ -582,7 +662,7 @@ __global__ void __launch_bounds__(128) gn_fold_moments_kernel(const float2* __re
 
 // y = act((x - mean) rstd gamma + beta)
 template <int DT, int ACT, bool kRagged>
-__global__ void __launch_bounds__(512) gn_apply_kernel(const void* __restrict__ x, void* __restrict__ y, const float* __restrict__ gamma,
+__global__ void __launch_bounds__(512, 1) gn_apply_kernel(const void* __restrict__ x, void* __restrict__ y, const float* __restrict__ gamma,
                                                        const float* __restrict__ beta, const float* __restrict__ mean,
                                                        const float* __restrict__ rstd, GnGeom g) {
   constexpr int V = Elem<DT>::V, H = V / 2;
@@ -601,12 +681,15 @@ __global__ void __launch_bounds__(512) gn_apply_kernel(const void* __restrict__ 
     f.be[i] = pk(beta[c[2 * i]], beta[c[2 * i + 1]]);
   }
   const int pitch = g.W / V;
-  const uint4* src = reinterpret_cast<const uint4*>(x) + (h.f0 + lane) * pitch + vcol;
+  extern __shared__ float4 ring4[];
+  const uint4* src[1] = {reinterpret_cast<const uint4*>(x) + (h.f0 + lane) * pitch + vcol};
   uint4* dst = reinterpret_cast<uint4*>(y) + (h.f0 + lane) * pitch + vcol;
   const int rows = (int)max(0ll, h.f1 - h.f0 - lane);
   const size_t step = (size_t)g.lanes * pitch;
-#pragma unroll 4
-  for (int r = 0; r < rows; r += g.lanes, src += step, dst += step) __stcs(dst, f(__ldcs(src)));
+  stream_vectors<1>(src, step, (rows + g.lanes - 1) / g.lanes, reinterpret_cast<uint4*>(ring4), [&](int, const uint4 (&v)[1]) {
+    __stcs(dst, f(v[0]));
+    dst += step;
+  });
   if (kRagged)
     edge_rows(g, h, lane, [&](long long row) {
       const long long e = row * g.W + (long long)vcol * V;
@@ -616,11 +699,11 @@ __global__ void __launch_bounds__(512) gn_apply_kernel(const void* __restrict__ 
 
 // part[n][slice][0..1][e] = sums over the slice's column e of g and of g xh
 template <int DT, int ACT, bool kRagged>
-__global__ void __launch_bounds__(512) gn_grad_sums_kernel(const void* __restrict__ dy, const void* __restrict__ x, const float* __restrict__ gamma,
+__global__ void __launch_bounds__(512, 1) gn_grad_sums_kernel(const void* __restrict__ dy, const void* __restrict__ x, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, const float* __restrict__ mean,
                                                            const float* __restrict__ rstd, float* __restrict__ part, GnGeom g) {
-  constexpr int V = Elem<DT>::V, H = V / 2, U = 2;
-  extern __shared__ float sh[];
+  constexpr int V = Elem<DT>::V, H = V / 2;
+  extern __shared__ float sh[];        // the ring, then the folds' space
   float* red = sh;
   float* tree = red + blockDim.x * V;
   float* col = tree + blockDim.x;
@@ -636,25 +719,13 @@ __global__ void __launch_bounds__(512) gn_grad_sums_kernel(const void* __restric
     f.load(g, n, c, gamma, beta, mean, rstd);
     const int pitch = g.W / V;
     const size_t at = (size_t)(h.f0 + lane) * pitch + vcol, step = (size_t)g.lanes * pitch;
-    const uint4* px = reinterpret_cast<const uint4*>(x) + at;
-    const uint4* pd = reinterpret_cast<const uint4*>(dy) + at;
+    const uint4* src[2] = {reinterpret_cast<const uint4*>(x) + at, reinterpret_cast<const uint4*>(dy) + at};
     const int rows = (int)max(0ll, h.f1 - h.f0 - lane);
     f2 xh[H], t[H];
-    int r = 0;
-    for (; r + (U - 1) * g.lanes < rows; r += U * g.lanes, px += U * step, pd += U * step) {
-      uint4 vx[U], vd[U];
-#pragma unroll
-      for (int k = 0; k < U; ++k) { vx[k] = px[k * step]; vd[k] = pd[k * step]; }
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        f(vx[k], vd[k], xh, t);
-        sum.add(xh, t);
-      }
-    }
-    for (; r < rows; r += g.lanes, px += step, pd += step) {
-      f(px[0], pd[0], xh, t);
+    stream_vectors<2>(src, step, (rows + g.lanes - 1) / g.lanes, reinterpret_cast<uint4*>(sh), [&](int, const uint4 (&v)[2]) {
+      f(v[0], v[1], xh, t);
       sum.add(xh, t);
-    }
+    });
     if (kRagged)
       edge_rows(g, h, lane, [&](long long row) {
         const long long e = row * g.W + (long long)vcol * V;
@@ -662,72 +733,87 @@ __global__ void __launch_bounds__(512) gn_grad_sums_kernel(const void* __restric
         sum.add_edge(xh, t, e, h.lo, h.hi);
       });
   }
-  const int w = g.cols * V;
-  float* out = part + ((size_t)n * gridDim.x + blockIdx.x) * 2 * (size_t)(g.nblk * w) + (size_t)blk * w;
+  // columns of the slice; where one CTA has them all the f places of a channel meet here
+  const int w = g.cols * V, channels = g.nblk == 1 ? g.C : w, pitch = g.nblk == 1 ? g.C : g.nblk * w;
+  float* out = part + ((size_t)n * gridDim.x + blockIdx.x) * 2 * (size_t)pitch + (size_t)blk * w;
   float v[V];
   GradSums<DT, ACT>::unpack(sum.b, v);
-  column_sums<V>(g, v, j, lane, red, tree, col);
-  for (int e = threadIdx.x; e < w; e += blockDim.x) out[e] = col[e];
-  __syncthreads();
-  GradSums<DT, ACT>::unpack(sum.w, v);
-  column_sums<V>(g, v, j, lane, red, tree, col);
-  for (int e = threadIdx.x; e < w; e += blockDim.x) out[(size_t)g.nblk * w + e] = col[e];
-}
-
-// Channel sums of a picture, nc[n][0..1][c], and the two means of each of its groups, coef[n][k] = (m1, m2).
-// One CTA of 256 threads per (picture, group).
-__global__ void __launch_bounds__(256) gn_fold_grads_kernel(const float* __restrict__ part, const float* __restrict__ gamma, float* __restrict__ nc,
-                                                            float2* __restrict__ coef, GnGeom g, int slices, int pitch) {
-  __shared__ float sh[2][8];
-  const int n = blockIdx.x / g.G, k = blockIdx.x % g.G;
-  const int warp = threadIdx.x >> 5, ln = threadIdx.x & 31;
-  float m[2] = {0.0f, 0.0f};
-  // a warp per channel: its lanes add the slices
-  for (int cc = warp; cc < g.cpg; cc += 8) {
-    const int c = k * g.cpg + cc;
+  __syncthreads();                     // every thread is through with its ring
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float s = 0.0f;
-      for (int i = ln; i < slices * g.f; i += 32) {
-        const int sl = i / g.f, r = i - sl * g.f;
-        s += part[(((size_t)n * slices + sl) * 2 + h) * pitch + (size_t)r * g.C + c];
-      }
-      s = warp_sum(s);
-      if (ln == 0) nc[((size_t)n * 2 + h) * g.C + c] = s;
-      m[h] = fmaf(gamma[c], s, m[h]);
+  for (int half = 0; half < 2; ++half) {
+    column_sums<V>(g, v, j, lane, red, tree, col);
+    for (int e = threadIdx.x; e < channels; e += blockDim.x) {
+      float s = col[e];
+      if (g.nblk == 1)
+        for (int k = 1; k < g.f; ++k) s += col[e + k * g.C];
+      out[(size_t)half * pitch + e] = s;
     }
-  }
-  if (ln == 0) { sh[0][warp] = m[0]; sh[1][warp] = m[1]; }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float a = 0.0f, b = 0.0f;
-    for (int i = 0; i < 8; ++i) { a += sh[0][i]; b += sh[1][i]; }
-    coef[blockIdx.x] = make_float2(a * g.inv_count, b * g.inv_count);
+    __syncthreads();
+    GradSums<DT, ACT>::unpack(sum.w, v);
   }
 }
 
-// dgamma[c] = sum over pictures of nc[n][1][c], dbeta[c] of nc[n][0][c]; 32 channels x 32 picture lanes per CTA
-__global__ void __launch_bounds__(1024) gn_param_grads_kernel(const float* __restrict__ nc, float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                              int N, int C) {
+// Channel sums of a picture, nc[n][0..1][c], from the slices': 32 channels x 32 slice lanes per CTA.
+__global__ void __launch_bounds__(1024) gn_fold_grads_kernel(const float* __restrict__ part, float* __restrict__ nc, GnGeom g, int slices, int pitch) {
   __shared__ float sh[32][33];
-  const int i = blockIdx.x * 32 + threadIdx.x;   // over [2][C]
+  const int n = blockIdx.y, i = blockIdx.x * 32 + threadIdx.x, h = i >= g.C ? 1 : 0, c = i - h * g.C;   // over [2][C]
   float s = 0.0f;
-  if (i < 2 * C)
-    for (int n = threadIdx.y; n < N; n += 32) s += nc[(size_t)n * 2 * C + i];
+  if (i < 2 * g.C) {
+    const float* p = part + ((size_t)n * slices * 2 + h) * pitch + c;
+    const int places = g.nblk == 1 ? 1 : g.f;
+#pragma unroll 4
+    for (int sl = threadIdx.y; sl < slices; sl += 32)
+      for (int k = 0; k < places; ++k) s += p[(size_t)sl * 2 * pitch + (size_t)k * g.C];
+  }
   sh[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && i < 2 * C) {
+  if (threadIdx.y == 0 && i < 2 * g.C) {
     float t = 0.0f;
 #pragma unroll
     for (int r = 0; r < 32; ++r) t += sh[r][threadIdx.x];
-    if (i < C) dbeta[i] = t;
-    else dgamma[i - C] = t;
+    nc[(size_t)n * 2 * g.C + i] = t;
+  }
+}
+
+// dgamma[c] = sum over pictures of nc[n][1][c], dbeta[c] of nc[n][0][c]: 32 channels x 32 picture lanes per CTA.  CTAs behind
+// the first `param_ctas`: the two means of the groups, coef[n][k] = (m1, m2), one warp each.
+__global__ void __launch_bounds__(1024) gn_param_grads_kernel(const float* __restrict__ nc, float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                              const float* __restrict__ gamma, float2* __restrict__ coef, GnGeom g, int param_ctas) {
+  __shared__ float sh[32][33];
+  if ((int)blockIdx.x >= param_ctas) {
+    const int k = ((int)blockIdx.x - param_ctas) * 32 + threadIdx.y;   // (picture, group)
+    if (k >= g.N * g.G) return;
+    const int n = k / g.G, c0 = (k - n * g.G) * g.cpg;
+    const float* b = nc + (size_t)n * 2 * g.C + c0;
+    float m1 = 0.0f, m2 = 0.0f;
+    for (int c = threadIdx.x; c < g.cpg; c += 32) {
+      const float w = gamma[c0 + c];
+      m1 = fmaf(w, b[c], m1);
+      m2 = fmaf(w, b[g.C + c], m2);
+    }
+    m1 = warp_sum(m1);
+    m2 = warp_sum(m2);
+    if (threadIdx.x == 0) coef[k] = make_float2(m1 * g.inv_count, m2 * g.inv_count);
+    return;
+  }
+  const int i = blockIdx.x * 32 + threadIdx.x;   // over [2][C]
+  float s = 0.0f;
+  if (i < 2 * g.C)
+    for (int n = threadIdx.y; n < g.N; n += 32) s += nc[(size_t)n * 2 * g.C + i];
+  sh[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && i < 2 * g.C) {
+    float t = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) t += sh[r][threadIdx.x];
+    if (i < g.C) dbeta[i] = t;
+    else dgamma[i - g.C] = t;
   }
 }
 
 // dx = rstd (gamma g - m1 - xh m2)
 template <int DT, int ACT, bool kRagged>
-__global__ void __launch_bounds__(512) gn_grad_apply_kernel(const void* __restrict__ dy, const void* __restrict__ x, void* __restrict__ dx,
+__global__ void __launch_bounds__(512, 1) gn_grad_apply_kernel(const void* __restrict__ dy, const void* __restrict__ x, void* __restrict__ dx,
                                                             const float* __restrict__ gamma, const float* __restrict__ beta,
                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
                                                             const float2* __restrict__ coef, GnGeom g) {
@@ -749,16 +835,16 @@ __global__ void __launch_bounds__(512) gn_grad_apply_kernel(const void* __restri
   a.set(f, m1, m2);
   const int pitch = g.W / V;
   const size_t at = (size_t)(h.f0 + lane) * pitch + vcol, step = (size_t)g.lanes * pitch;
-  const uint4* px = reinterpret_cast<const uint4*>(x) + at;
-  const uint4* pd = reinterpret_cast<const uint4*>(dy) + at;
+  extern __shared__ float4 ring4[];
+  const uint4* src[2] = {reinterpret_cast<const uint4*>(x) + at, reinterpret_cast<const uint4*>(dy) + at};
   uint4* dst = reinterpret_cast<uint4*>(dx) + at;
   const int rows = (int)max(0ll, h.f1 - h.f0 - lane);
   f2 xh[H], t[H];
-#pragma unroll 2
-  for (int r = 0; r < rows; r += g.lanes, px += step, pd += step, dst += step) {
-    f(__ldcs(px), __ldcs(pd), xh, t);
+  stream_vectors<2>(src, step, (rows + g.lanes - 1) / g.lanes, reinterpret_cast<uint4*>(ring4), [&](int, const uint4 (&v)[2]) {
+    f(v[0], v[1], xh, t);
     __stcs(dst, a(xh, t));
-  }
+    dst += step;
+  });
   if (kRagged)
     edge_rows(g, h, lane, [&](long long row) {
       const long long e = row * g.W + (long long)vcol * V;
@@ -788,18 +874,6 @@ __device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
   return v;
 }
 
-// 16 bytes from global to shared memory without passing through registers; a thread reads only what it copied itself
-__device__ __forceinline__ void copy16(const void* dst_shared, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst_shared)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// waits until at most `n` of the thread's latest groups are in flight
-__device__ __forceinline__ void copy_wait(int n) {
-  if (n >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
-  else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
-  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-  else asm volatile("cp.async.wait_group 0;" ::: "memory");
-}
 constexpr int kPieces = 4;   // a thread's vectors arrive in this many groups
 
 // A cluster's place: grid (cluster size, column blocks, pictures).
@@ -1358,23 +1432,29 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
     HE_TRY(limit.raise(kernel, ctx->device, kMaxSmem));
     HE_CUDA(cudaLaunchKernelEx(&lc, kernel, in[0], in[1], out[0], (const float*)in[2], (const float*)in[3], (const float*)in[4],
                                (const float*)in[5], (float*)ws, g));
-    gn_param_grads_kernel<<<(2 * g.C + 31) / 32, dim3(32, 32), 0, st>>>((const float*)ws, (float*)out[1], (float*)out[2], g.N, g.C);
+    const int param_ctas = (2 * g.C + 31) / 32;
+    gn_param_grads_kernel<<<param_ctas, dim3(32, 32), 0, st>>>((const float*)ws, (float*)out[1], (float*)out[2], nullptr, nullptr, g, param_ctas);
     HE_CUDA(cudaGetLastError());
     last_launches = 2;
     return HE_OK;
   }
   const dim3 grid((unsigned)slices, (unsigned)g.nblk, (unsigned)g.N);
   const int w = g.cols * V, pitch = g.nblk * w;
-  const size_t smem = (size_t)(threads * V + threads + w) * sizeof(float);
+  const int tensors = direction == HE_GN_FORWARD ? 1 : 2;
+  const size_t ring = (size_t)kDepth * tensors * threads * 16, folds = (size_t)(threads * V + threads + w + g.G) * sizeof(float);
+  const size_t smem = std::max(ring, folds);
+  static SmemLimit limits2[4];
   if (direction == HE_GN_FORWARD) {
     const void* x = in[0];
     const float* gamma = (const float*)in[1]; const float* beta = (const float*)in[2];
     float* mean = (float*)out[1]; float* rstd = (float*)out[2];
+    HE_TRY(limits2[0].raise(gn_moments_kernel<DT, R>, ctx->device, kMaxSmem));
+    HE_TRY(limits2[1].raise(gn_apply_kernel<DT, ACT, R>, ctx->device, kMaxSmem));
     gn_moments_kernel<DT, R><<<grid, threads, smem, st>>>(x, (float2*)ws, g);
     HE_CUDA(cudaGetLastError());
-    gn_fold_moments_kernel<<<g.N * g.G, 128, 0, st>>>((const float2*)ws, mean, rstd, g, slices, pitch);
+    gn_fold_moments_kernel<<<g.N * g.G, 256, 0, st>>>((const float2*)ws, mean, rstd, g, slices, pitch);
     HE_CUDA(cudaGetLastError());
-    gn_apply_kernel<DT, ACT, R><<<grid, threads, 0, st>>>(x, out[0], gamma, beta, mean, rstd, g);
+    gn_apply_kernel<DT, ACT, R><<<grid, threads, ring, st>>>(x, out[0], gamma, beta, mean, rstd, g);
     HE_CUDA(cudaGetLastError());
     last_launches = 3;
     return HE_OK;
@@ -1384,13 +1464,16 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
   float* nc = (float*)ws;                                         // [N][2][C]
   float2* coef = (float2*)(nc + (size_t)g.N * 2 * g.C);           // [N][G]
   float* part = (float*)(coef + (size_t)g.N * g.G);               // [N][slices][2][pitch]
+  HE_TRY(limits2[2].raise(gn_grad_sums_kernel<DT, ACT, R>, ctx->device, kMaxSmem));
+  HE_TRY(limits2[3].raise(gn_grad_apply_kernel<DT, ACT, R>, ctx->device, kMaxSmem));
   gn_grad_sums_kernel<DT, ACT, R><<<grid, threads, smem, st>>>(in[0], in[1], gamma, beta, mean, rstd, part, g);
   HE_CUDA(cudaGetLastError());
-  gn_fold_grads_kernel<<<g.N * g.G, 256, 0, st>>>(part, gamma, nc, coef, g, slices, pitch);
+  const int param_ctas = (2 * g.C + 31) / 32, coef_ctas = (g.N * g.G + 31) / 32;
+  gn_fold_grads_kernel<<<dim3((unsigned)param_ctas, (unsigned)g.N), dim3(32, 32), 0, st>>>(part, nc, g, slices, g.nblk == 1 ? g.C : pitch);
   HE_CUDA(cudaGetLastError());
-  gn_param_grads_kernel<<<(2 * g.C + 31) / 32, dim3(32, 32), 0, st>>>(nc, (float*)out[1], (float*)out[2], g.N, g.C);
+  gn_param_grads_kernel<<<param_ctas + coef_ctas, dim3(32, 32), 0, st>>>(nc, (float*)out[1], (float*)out[2], gamma, coef, g, param_ctas);
   HE_CUDA(cudaGetLastError());
-  gn_grad_apply_kernel<DT, ACT, R><<<grid, threads, 0, st>>>(in[0], in[1], out[0], gamma, beta, mean, rstd, coef, g);
+  gn_grad_apply_kernel<DT, ACT, R><<<grid, threads, ring, st>>>(in[0], in[1], out[0], gamma, beta, mean, rstd, coef, g);
   HE_CUDA(cudaGetLastError());
   last_launches = 4;
   return HE_OK;
@@ -1504,6 +1587,11 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
       }
     }
   }
+  // Against two passes over all of it (three launches forward, four backward, 5.6 TB/s): worth it for the largest tensors
+  // only, where the slabs' folds and exchanges add up ([64,3136,256] bf16: backward 105 us in two passes, 129 us in slabs,
+  // forward 73 and 52 us; [128,784,128] backward 41 and 33 us).
+  const double two_us = (fwd ? 18.0 : 22.0) + (double)g.total * es * (fwd ? 3 : 5) / 5.6e6;
+  if (plan->cluster && 6.0 + 1.25 * best > two_us) plan->cluster = 0;
   if (plan->cluster) {
     g.lanes = plan->threads / g.cols;
     plan->workspace_bytes = direction == HE_GN_FORWARD ? 0 : (size_t)g.N * 2 * g.C * sizeof(float);
@@ -1514,19 +1602,22 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
     *out = plan.release();
     return HE_OK;
   }
+  // Two passes: CTAs of 256 threads, or as many more as a row's vectors take
+  plan->threads = vcols > 256 ? 512 : 256;
   g.cols = std::min(vcols, plan->threads);
   g.nblk = (vcols + g.cols - 1) / g.cols;
   g.lanes = plan->threads / g.cols;
-  // slices: about four CTAs of 512 threads for each SM, at least 16 super-rows a thread (the folds' cost is per CTA)
+  // slices: what lives on the SMs at once (shared memory holds the rings of 6 CTAs forward, 3 backward), at least 16
+  // super-rows a thread (the folds' cost is per CTA)
   const long long per_min = (long long)g.lanes * 16;
-  long long want = std::max<long long>(1, (long long)sms * 4 / std::max<long long>(1, (long long)g.N * g.nblk));
+  long long want = std::max<long long>(1, (long long)sms * (fwd ? 6 : 3) * 256 / plan->threads / std::max<long long>(1, (long long)g.N * g.nblk));
   want = std::min(want, std::max<long long>(1, srows / per_min));
   g.per = (int)((srows + want - 1) / want);
   plan->slices = (int)((srows + g.per - 1) / g.per);
-  const size_t pitch = (size_t)g.nblk * g.cols * V;
-  plan->workspace_bytes = direction == HE_GN_FORWARD
-                              ? (size_t)g.N * plan->slices * pitch * sizeof(float2)
-                              : ((size_t)g.N * 2 * g.C + (size_t)g.N * g.G * 2 + (size_t)g.N * plan->slices * 2 * pitch) * sizeof(float);
+  // partial sums of a slice: of the groups or the channels, or of all columns where they are cut into blocks
+  const size_t columns = (size_t)g.nblk * g.cols * V;
+  plan->workspace_bytes = fwd ? (size_t)g.N * plan->slices * (g.nblk == 1 ? g.G : columns) * sizeof(float2)
+                              : ((size_t)g.N * 2 * g.C + (size_t)g.N * g.G * 2 + (size_t)g.N * plan->slices * 2 * (g.nblk == 1 ? g.C : columns)) * sizeof(float);
   snprintf(desc, sizeof desc, "group norm %s: %s [%d,%d,%d] in %d groups, activation %s, two passes over %d slices a picture",
            direction == HE_GN_FORWARD ? "forward" : "backward", dtype_name(prm->dtype), g.N, g.P, g.C, g.G, kActs[plan->act], plan->slices);
   plan->description = desc;
