@@ -83,6 +83,32 @@ pub const HE_CONV_FWD: i32 = 0;
 pub const HE_CONV_BWD_DATA: i32 = 1;
 pub const HE_CONV_BWD_FILTER: i32 = 2;
 
+pub const HE_GN_FORWARD: i32 = 0;
+pub const HE_GN_BACKWARD: i32 = 1;
+pub const HE_ACT_NONE: i32 = 0;
+pub const HE_ACT_RELU: i32 = 1;
+pub const HE_ACT_SILU: i32 = 2;
+pub const HE_ACT_GELU: i32 = 3;
+
+#[repr(C)]
+#[derive(Copy, Clone)]
+pub struct he_group_norm_params {
+    pub batch: i32, pub channels: i32,
+    pub positions: i64,
+    pub groups: i32, pub dtype: i32, pub activation: i32,
+    pub eps: f32,
+}
+
+#[repr(C)]
+#[derive(Copy, Clone)]
+pub struct he_muon_params {
+    pub count: i32,
+    pub rows: *const i64, pub cols: *const i64, pub scales: *const f32,
+    pub grad_dtype: i32, pub out_dtype: i32, pub steps: i32,
+    pub coef: [f32; 3], pub eps: f32,
+    pub use_momentum: i32, pub momentum: f32, pub nesterov: i32,
+}
+
 #[repr(C)]
 pub struct he_graph_desc {
     pub num_nodes: i32,
@@ -122,6 +148,8 @@ extern "C" {
 
     pub fn he_plan_conv2d(ctx: *mut he_ctx, kind: i32, params: *const he_conv2d_params, batch: i32, in_h: i32, in_w: i32,
                           dtype: i32, fusion: *const he_conv2d_fusion, out: *mut *mut he_plan) -> i32;
+    pub fn he_plan_group_norm(ctx: *mut he_ctx, direction: i32, params: *const he_group_norm_params, out: *mut *mut he_plan) -> i32;
+    pub fn he_plan_muon(ctx: *mut he_ctx, params: *const he_muon_params, out: *mut *mut he_plan) -> i32;
     pub fn he_bn_finalize(stats: *const f32, count: i64, gamma: *const f32, beta: *const f32, running_mean: *mut f32,
                           running_var: *mut f32, scale: *mut f32, shift: *mut f32, mean: *mut f32, rstd: *mut f32, channels: i32,
                           cu_stream: *mut c_void) -> i32;
