@@ -1441,7 +1441,7 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
   const dim3 grid((unsigned)slices, (unsigned)g.nblk, (unsigned)g.N);
   const int w = g.cols * V, pitch = g.nblk * w;
   const int tensors = direction == HE_GN_FORWARD ? 1 : 2;
-  const size_t ring = (size_t)kDepth * tensors * threads * 16, folds = (size_t)(threads * V + threads + w + g.G) * sizeof(float);
+  const size_t ring = (size_t)kDepth * tensors * threads * 16, folds = (size_t)(threads * V + threads + w + (g.nblk == 1 ? g.G : 0)) * sizeof(float);
   const size_t smem = std::max(ring, folds);
   static SmemLimit limits2[4];
   if (direction == HE_GN_FORWARD) {

@@ -141,6 +141,17 @@ def test_backward(ctx, size, dt):
         assert bool((err <= tol).all()), (plan.description, float((err / tol).max()))
 
 
+# A group per channel beyond what shared memory could list; columns are cut into blocks there, forward and backward alike.
+MANY_GROUPS = [(1, 4, 65535, 65535), (2, 3, 50001, 50001), (1, 4, 65536, 65536)]
+
+
+@pytest.mark.parametrize("dt", [ir.BF16, ir.F32])
+@pytest.mark.parametrize("size", MANY_GROUPS)
+def test_many_groups(ctx, size, dt):
+    test_forward(ctx, size, dt)
+    test_backward(ctx, size, dt)
+
+
 @pytest.mark.parametrize("act", ["none", "silu", "gelu"])
 def test_backward_against_differences(ctx, act):
     """d/dt of sum(w y) along random directions of x, gamma and beta: central differences of the 64-bit forward."""
