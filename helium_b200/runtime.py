@@ -290,7 +290,7 @@ class Plan:
             target = torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream
             with torch.cuda.stream(target):
                 return self._launch_on(torch, target.cuda_stream, dev, inputs, ins, outputs)
-        return self._launch_on(torch, torch.cuda.current_stream(dev).cuda_stream, dev, inputs, ins, outputs)
+        return self._launch_on(torch, torch._C._cuda_getCurrentRawStream(dev), dev, inputs, ins, outputs)
 
     def _launch_on(self, torch, stream_ptr, dev, inputs, ins, outputs):
         _, out_specs, sources, ws_bytes, in_array, out_array = self._torch_specs
