@@ -1487,17 +1487,25 @@ int32_t GroupNormPlan::launch(const void* const* in, void* const* out, void* ws,
   for (int i = 0; i < 3; ++i)
     if (!out[i]) HE_FAIL(HE_ERR_INVALID, "group norm: output %d is null", i);
   const int n_big = direction == HE_GN_FORWARD ? 1 : 2;
-  const size_t bytes = (size_t)g.total * dtype_bytes(dtype);
-  const uintptr_t o = (uintptr_t)out[0];
-  for (int i = 0; i < n_big; ++i) {
-    const uintptr_t p = (uintptr_t)in[i];
-    if (p & 15) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: tensors must be 16-byte aligned");
-    if (p < o + bytes && o < p + bytes) HE_FAIL(HE_ERR_INVALID, "group norm: the output overlaps input %d", i);
+  // No output overlaps an input or another output: later kernels of a launch read what earlier ones would have written over.
+  const size_t big = (size_t)g.total * dtype_bytes(dtype), param = (size_t)g.C * 4, stat = (size_t)g.N * g.G * 4;
+  auto in_bytes = [&](int i) { return i < n_big ? big : i < n_big + 2 ? param : stat; };
+  auto out_bytes = [&](int i) { return i == 0 ? big : direction == HE_GN_FORWARD ? stat : param; };
+  auto meet = [](const void* p, size_t np, const void* q, size_t nq) {
+    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+  };
+  for (int o = 0; o < 3; ++o) {
+    for (int i = 0; i < n_in; ++i)
+      if (meet(out[o], out_bytes(o), in[i], in_bytes(i))) HE_FAIL(HE_ERR_INVALID, "group norm: output %d overlaps input %d", o, i);
+    for (int i = 0; i < o; ++i)
+      if (meet(out[o], out_bytes(o), out[i], out_bytes(i))) HE_FAIL(HE_ERR_INVALID, "group norm: output %d overlaps output %d", o, i);
   }
-  if (o & 15) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: tensors must be 16-byte aligned");
+  for (int i = 0; i < n_big; ++i)
+    if ((uintptr_t)in[i] & 15) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: tensors must be 16-byte aligned");
+  if ((uintptr_t)out[0] & 15) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: tensors must be 16-byte aligned");
   for (int i = n_big; i < n_in; ++i) {
-    const bool param = i < n_big + 2;   // gamma and beta are read as vectors
-    if ((uintptr_t)in[i] & (param ? 15 : 3)) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: %s must be %d-byte aligned", param ? "gamma and beta" : "mean and rstd", param ? 16 : 4);
+    const bool vectors = i < n_big + 2;   // gamma and beta are read as vectors
+    if ((uintptr_t)in[i] & (vectors ? 15 : 3)) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: %s must be %d-byte aligned", vectors ? "gamma and beta" : "mean and rstd", vectors ? 16 : 4);
   }
   if (((uintptr_t)out[1] | (uintptr_t)out[2]) & 3) HE_FAIL(HE_ERR_UNSUPPORTED, "group norm: f32 vectors must be 4-byte aligned");
   switch (dtype) {

@@ -352,8 +352,8 @@ int32_t he_plan_conv2d(he_ctx* ctx, int32_t kind, const he_conv2d_params* params
  *                   outputs y, mean f32 [batch, groups], rstd f32 [batch, groups]
  *   HE_GN_BACKWARD  inputs  dy, x, gamma, beta, mean, rstd (the forward pass's)
  *                   outputs dx, dgamma f32 [C], dbeta f32 [C] (summed over batch and positions)
- * x, y, dy, dx have `dtype` (F16 / BF16 / F32); they, gamma and beta start on 16-byte boundaries; y and dx overlap no
- * input; any sizes from one position and one channel on.  Sums and statistics are f32, taken in a fixed order: results
+ * x, y, dy, dx have `dtype` (F16 / BF16 / F32); they, gamma and beta start on 16-byte boundaries; no output overlaps
+ * an input or another output; any sizes from one position and one channel on.  Sums and statistics are f32, taken in a fixed order: results
  * repeat bit for bit.  The rectifier's derivative at 0 is 0.  A group that holds a NaN or an infinity comes out as NaN.
  * ------------------------------------------------------------------------------------------------ */
 typedef enum he_activation { HE_ACT_NONE = 0, HE_ACT_RELU = 1, HE_ACT_SILU = 2, HE_ACT_GELU = 3 /* exact erf form */ } he_activation;

@@ -322,3 +322,24 @@ def test_refused_launches(ctx):
     big = torch.empty(plan.workspace_bytes + 256, dtype=torch.uint8, device="cuda")
     rc = lib.he_launch(plan._h, ins, outs, C.c_void_p((big.data_ptr() + 255) // 256 * 256), C.c_void_p(torch.cuda.current_stream().cuda_stream))
     assert rc == -1 and b"input 1 is null" in lib.he_last_error_string()
+
+
+@pytest.mark.parametrize("p", [10, 300000])   # one pass and two
+def test_outputs_that_overlap_are_refused(ctx, p):
+    import torch
+    n, c, groups = 1, 16, 16
+    x, gamma, beta, dy = _inputs(n, p, c, ir.BF16, 1)
+    st = lambda: torch.ones(n, groups, device="cuda")  # noqa: E731
+    vec = lambda: torch.ones(c, device="cuda")  # noqa: E731
+    fwd = hb.Plan.group_norm(ctx, "fwd", n, p, c, groups)
+    s = st()
+    for outs in ([x, st(), st()], [torch.empty_like(x), s, s], [torch.empty_like(x), st(), gamma.view(n, groups)],
+                 [torch.empty_like(x), beta.view(n, groups), st()]):
+        with pytest.raises(hb.HeliumError, match="overlaps"):
+            fwd.launch([x, gamma, beta], outs)
+    bwd = hb.Plan.group_norm(ctx, "bwd", n, p, c, groups)
+    mean, rstd, v = st(), st(), vec()
+    for outs in ([x, vec(), vec()], [dy, vec(), vec()], [torch.empty_like(x), gamma, vec()], [torch.empty_like(x), vec(), beta],
+                 [torch.empty_like(x), v, v], [torch.empty_like(x), mean.view(c), vec()]):
+        with pytest.raises(hb.HeliumError, match="overlaps"):
+            bwd.launch([dy, x, gamma, beta, mean, rstd], outs)
