@@ -10,9 +10,10 @@
 // matrices, of which the symmetric ones (S and S^2) compute the tiles on and below the diagonal only.
 //
 // Numbers.  The operands are f16, each matrix scaled by a power of two: X by sx ~ sqrt(m n), which makes its
-// root-mean-square 1 at the start and keeps |X| below 65504 (|X| <= 1.3 sx), S by 2^12, B by 2^10.  X itself is kept as a
-// pair hi + lo of f16 (22 bits): the products read hi, the term a X adds the pair, so the rounding of hi is not multiplied
-// by a = 3.4 step after step, and B's diagonal, by far its largest values, stays f32 and is applied to the pair too.
+// root-mean-square 1 at the start and keeps |X| below 65504 (|X| <= 1.3 sx with the usual coefficients; others are checked
+// when a call is planned), S by 2^12, B by 2^10.  X itself is kept as a pair hi + lo of f16 (22 bits): the products read
+// hi, the term a X adds the pair, so the rounding of hi is not multiplied by a = 3.4 step after step, and B's diagonal, by
+// far its largest values, stays f32 and is applied to the pair too.
 // Simulated against 64 bits, the update is 4e-4 .. 9e-4 off (relative, 2-norm), half a bf16 rounding of the result;
 // bf16 operands were 4e-3 .. 2e-2 off, f16 without the pair 2e-3 .. 5e-3.
 //
@@ -296,9 +297,9 @@ __global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ 
 // tiles (350 ns for the 32 KB of a 64-deep block, 13.5 TB/s over the chip, where the products take 140 ns).
 //
 // Warps: 0 items and loads, 1 products, 2 and 3 stores, 4 .. 19 epilogue: four teams of four warps, each on 32 of every 128
-// columns.  Behind a
-// tile's operands the same ring hands the epilogue one stage for every 64 columns: TMA brings what it reads there (S, or X's
-// two halves), the results replace it in place and TMA takes them out, the mirrored tile of a symmetric product too.
+// columns.  Behind a tile's operands the same ring hands the epilogue one stage for every 64 columns: TMA brings what it
+// reads there (S, or X's two halves), the results replace it in place and TMA takes them out, the mirrored tile of a
+// symmetric product too.
 // What follows a store (its completion, the count) is the store warps' business: an epilogue that waited for them itself took
 // 5.8 us a tile of the conv net's X, whose products take 3.8.
 // (A thread owns a row.  Its own 32-byte loads and stores touch a line of its own each: 6 us a 128 x 128 tile with both, 3.2 us
@@ -1387,6 +1388,18 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     if (!std::isfinite(prm->coef[i])) HE_FAIL(HE_ERR_INVALID, "muon: coefficients must be finite");
   if (!(prm->eps >= 0.0f) || !std::isfinite(prm->eps)) HE_FAIL(HE_ERR_INVALID, "muon: eps must be finite and not negative");
   if (!(prm->momentum >= 0.0f && prm->momentum < 1.0f)) HE_FAIL(HE_ERR_INVALID, "muon: momentum must be in [0, 1)");
+  // The products' f16 operands have room for |X| < 65504 / 2^15 and |b S + c S^2| < 65504 / 2^10 (an entry is at most the
+  // largest singular value): the map of the singular values, which start in [0, 1], is followed step by step.
+  for (int i = 0; i <= 4096; ++i) {
+    double v = i / 4096.0;
+    for (int step = 0; step < prm->steps; ++step) {
+      const double q = v * v;
+      if (!(std::fabs(v) < 1.9) || !(std::fabs((double)prm->coef[1]) * q + std::fabs((double)prm->coef[2]) * q * q < 60.0))
+        HE_FAIL(HE_ERR_UNSUPPORTED, "muon: after %d steps these coefficients take a singular value of %.4f to %g, beyond the products' range", step,
+                i / 4096.0, v);
+      v = v * (prm->coef[0] + q * (prm->coef[1] + q * (double)prm->coef[2]));
+    }
+  }
   std::unique_ptr<MuonPlan> plan(new MuonPlan);
   plan->ctx = ctx;
   plan->count = prm->count;

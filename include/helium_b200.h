@@ -423,9 +423,10 @@ int32_t he_sgd_momentum(float* w, float* avg, const void* grad, int32_t grad_dty
  *   outputs  update of every matrix (out_dtype: BF16 or F16), then, with use_momentum, the new averages (f32; an output
  *            may be the input average itself, no other operands may overlap)
  * The products run on f16 operands with f32 accumulation: an update is about 1e-3 (2-norm, relative) from the same steps in
- * 64 bits; averages are f32.  `coef` must keep the singular values, which start in [0, 1], below 4.  The update is
- * applied by he_sgd_momentum with `avg` NULL.  One workspace serves one launch at a time.  Tensors start on 16-byte
- * boundaries; min(rows, cols) <= 32768. */
+ * 64 bits; averages are f32.  `coef` must keep every singular value v, which start in [0, 1], below 1.9 and
+ * |b| v^2 + |c| v^4 below 60 at the start of each step; others are refused.  With eps 0 a zero gradient gives NaN.  The
+ * update is applied by he_sgd_momentum with `avg` NULL.  One workspace serves one launch at a time.  Tensors start on
+ * 16-byte boundaries; min(rows, cols) <= 32768. */
 typedef struct he_muon_params {
   int32_t count;            /* matrices */
   const int64_t* rows;      /* [count] */

@@ -55,3 +55,22 @@ def test_refused_calls():
         hb.Plan.muon(None, [(4, 4)], scales=[1.0, 2.0])
     p = hb.Plan.muon(None, [(4, 4)], momentum=None)
     assert lib.he_launch(p._h, None, None, None, None) == -1      # planned without a context: no CPU path
+
+
+@pytest.mark.parametrize("coefs,steps,fits", [
+    ((3.4445, -4.775, 2.0315), 64, True), ((1.5, -0.5, 0.0), 64, True), ((1.875, -1.25, 0.375), 64, True), ((2.0, -1.5, 0.5), 64, True),
+    ((1.0, 0.0, 0.0), 64, True),
+    ((4.0, 0.0, 0.0), 1, True),          # the step itself starts inside the range, what it makes is only written out
+    ((4.0, 0.0, 0.0), 2, False),         # X past its f16 range
+    ((0.0, 70.0, -70.0), 1, False),      # B past its f16 range at once
+    ((3.4445, -4.775, 3.0), 5, False),   # runs away
+    ((3e38, -3e38, 3e38), 5, False),
+])
+def test_coefficients_that_leave_the_products_range_are_refused(coefs, steps, fits):
+    h = C.c_void_p()
+    rc = lib.he_plan_muon(None, C.byref(_params(coef=coefs, steps=steps)), C.byref(h))
+    assert (rc == 0) == fits, lib.he_last_error_string()
+    if fits:
+        lib.he_plan_destroy(h)
+    else:
+        assert rc == -2 and b"range" in lib.he_last_error_string() and not h.value

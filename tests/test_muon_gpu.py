@@ -153,6 +153,26 @@ def test_gradients_of_any_size(ctx, size):
     _check(o, want, _tolerance(ir.BF16, 5, g, eps=0.0), f"{size}")
 
 
+@pytest.mark.parametrize("shape", [(64, 64), (333, 257), (1024, 2048)])
+def test_a_gradient_of_one_entry(ctx, shape):
+    """The norm is one entry: X's largest value is as far from its root-mean-square as it can be.
+
+    Nothing averages over one value v, so half steps add up: X's high half twice in S and S itself are each 2^-11 off, 3 2^-11
+    in v^2 and twice that in v^4, so a step is |b| v^3 3 2^-11 + |c| v^5 6 2^-11 off (B's diagonal and the term a X are f32
+    and the pair's 2^-22), the later steps multiply that by their slopes, and the update is rounded once, 2^-8."""
+    import torch
+    g = torch.zeros(shape, device="cuda")
+    g[shape[0] // 2, 3] = -0.37
+    (o,) = hb.Plan.muon(ctx, [shape], grad_dtype=ir.F32, momentum=None).launch([g])
+    want, _ = _reference(g, None, None, False, 5)
+    (a, b, c), v, off = COEFS, 1.0, 0.0
+    for _ in range(5):
+        off = off * abs(a + 3 * b * v ** 2 + 5 * c * v ** 4) + (abs(b) * v ** 3 * 3 + abs(c) * v ** 5 * 6) * 2.0 ** -11
+        v = a * v + b * v ** 3 + c * v ** 5
+    _check(o, want, 2.0 ** -8 + 1.1 * off / v, f"{shape}")    # 1.1: second order, f32 roundings
+    assert int((o != 0).sum()) == 1
+
+
 def test_a_zero_gradient_gives_a_zero_update_and_nan_stays_in_its_matrix(ctx):
     import torch
     shapes = [(100, 200), (130, 70), (64, 64)]
