@@ -14,10 +14,11 @@
 // registers.  Where P is no multiple of f a super-row can hold the end of one picture and the start of the next:
 // elements outside the picture's range of whole rows are masked (kRagged).
 //
-// Sums are f32.  The forward moments are taken about a shift of each thread's own (the first value it sees): the
-// thread's sum of squares about the group mean m is then q - 2 d s + n d^2 with d = m - shift, whose cancellation is
-// bounded by the thread's own spread whatever the tensor's mean is, and partial moments of CTAs meet as
-// (count, mean, sum of squares about it) triples.  Every fold runs in a fixed order: results repeat bit for bit.
+// Sums are f32.  The forward moments are taken about a shift: in the two-pass kernels one of each thread's own (the first
+// value it sees), whose sums become the thread's about the group mean m by q - 2 d s + n d^2 with d = m - shift; in the slab
+// kernels the group's first value, and where that lies far from the mean a second round over the tile, which is on chip,
+// takes the mean instead.  Either way the cancellation is bounded whatever the tensor's mean is.  Every fold runs in a fixed
+// order: results repeat bit for bit.
 #include <algorithm>
 #include <cmath>
 #include <memory>
@@ -116,11 +117,15 @@ __device__ __forceinline__ f2 reciprocals(f2 v) {
   un(v, a, b);
   return pk(rcp(a), rcp(b));
 }
-// 1 / (1 + exp(-z)); exp overflows to infinity below z = -88, whose reciprocal is the 0 it should be
+// 1 / (1 + exp(-z)).  One reciprocal serves a pair, b / (a b) and a / (a b): the special-function unit, 8 cycles a warp, is all
+// but the bound here (two passes backward over a [2,512,512,128] tensor: 128 -> 121 us).  exp is held at 2^63 (z = -43.7) so
+// that the product is finite: below it the result is 1e-19.  (GELU, which waits for other things, was 2 % slower that way.)
 __device__ __forceinline__ f2 sigmoid2(f2 z) {
   float a, b;
   un(mul2(z, pk(-1.4426950408889634f, -1.4426950408889634f)), a, b);
-  return reciprocals(add2(pk(ex2(a), ex2(b)), pk(1.0f, 1.0f)));
+  un(add2(pk(ex2(fminf(a, 63.0f)), ex2(fminf(b, 63.0f))), pk(1.0f, 1.0f)), a, b);
+  const float r = rcp(a * b);
+  return mul2(pk(b, a), pk(r, r));
 }
 // Normal cumulative distribution, and exp(-z^2 / 2) beside it: half of erfc(|z| / sqrt 2) on the negative side (no
 // cancellation in the tail), one minus that on the other.  f32 tensors take the Chebyshev form of Numerical Recipes
