@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(512, 1) gn_moments_kernel(const void* __restri
   const int j = threadIdx.x % g.cols, lane = threadIdx.x / g.cols;
   const int vcol = blk * g.cols + j;
   const Share h = share_of(g, n, blockIdx.x);
+  ptx::grid_release();
   Moments<DT, kRagged> m;
   m.clear();
   if (lane < g.lanes && vcol * V < g.W) {
@@ -642,11 +643,12 @@ __global__ void __launch_bounds__(256) gn_fold_moments_kernel(const float2* __re
     const long long a = max(s0 * g.f, row0), b = min(s1 * g.f, row1);
     if (whole) {
       cnt = (float)max(0ll, b - a) * g.cpg;
-      return part[((size_t)n * slices + sl) * g.G + k];
+      return __ldcg(part + ((size_t)n * slices + sl) * g.G + k);
     }
     cnt = a < b ? (float)((b - kk + g.f - 1) / g.f - (a - kk + g.f - 1) / g.f) : 0.0f;
-    return part[((size_t)n * slices + sl) * pitch + (size_t)kk * g.C + (size_t)k * g.cpg + c];
+    return __ldcg(part + ((size_t)n * slices + sl) * pitch + (size_t)kk * g.C + (size_t)k * g.cpg + c);
   };
+  ptx::grid_wait();
   float s = 0.0f, cnt;
   for (int i = threadIdx.x; i < items; i += 256) s += item(i, cnt).x;
   const float m = block_sum(s) * g.inv_count;
@@ -715,6 +717,7 @@ __global__ void __launch_bounds__(512, 1) gn_grad_sums_kernel(const void* __rest
   const int n = blockIdx.z, blk = blockIdx.y;
   const int j = threadIdx.x % g.cols, lane = threadIdx.x / g.cols, vcol = blk * g.cols + j;
   const Share h = share_of(g, n, blockIdx.x);
+  ptx::grid_release();
   GradSums<DT, ACT> sum;
   sum.clear();
   if (lane < g.lanes && vcol * V < g.W) {
@@ -762,13 +765,15 @@ __global__ void __launch_bounds__(512, 1) gn_grad_sums_kernel(const void* __rest
 __global__ void __launch_bounds__(1024) gn_fold_grads_kernel(const float* __restrict__ part, float* __restrict__ nc, GnGeom g, int slices, int pitch) {
   __shared__ float sh[32][33];
   const int n = blockIdx.y, i = blockIdx.x * 32 + threadIdx.x, h = i >= g.C ? 1 : 0, c = i - h * g.C;   // over [2][C]
+  ptx::grid_release();
+  ptx::grid_wait();
   float s = 0.0f;
   if (i < 2 * g.C) {
     const float* p = part + ((size_t)n * slices * 2 + h) * pitch + c;
     const int places = g.nblk == 1 ? 1 : g.f;
 #pragma unroll 4
     for (int sl = threadIdx.y; sl < slices; sl += 32)
-      for (int k = 0; k < places; ++k) s += p[(size_t)sl * 2 * pitch + (size_t)k * g.C];
+      for (int k = 0; k < places; ++k) s += __ldcg(p + (size_t)sl * 2 * pitch + (size_t)k * g.C);
   }
   sh[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
@@ -785,6 +790,7 @@ __global__ void __launch_bounds__(1024) gn_fold_grads_kernel(const float* __rest
 __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const float* __restrict__ nc, float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                               const float* __restrict__ gamma, float2* __restrict__ coef, GnGeom g, int param_ctas) {
   __shared__ float sh[32][33];
+  ptx::grid_wait();
   if ((int)blockIdx.x >= param_ctas) {
     const int k = ((int)blockIdx.x - param_ctas) * 32 + threadIdx.y;   // (picture, group)
     if (k >= g.N * g.G) return;
@@ -793,8 +799,8 @@ __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const float* __res
     float m1 = 0.0f, m2 = 0.0f;
     for (int c = threadIdx.x; c < g.cpg; c += 32) {
       const float w = gamma[c0 + c];
-      m1 = fmaf(w, b[c], m1);
-      m2 = fmaf(w, b[g.C + c], m2);
+      m1 = fmaf(w, __ldcg(b + c), m1);
+      m2 = fmaf(w, __ldcg(b + g.C + c), m2);
     }
     m1 = warp_sum(m1);
     m2 = warp_sum(m2);
@@ -804,7 +810,7 @@ __global__ void __launch_bounds__(1024) gn_param_grads_kernel(const float* __res
   const int i = blockIdx.x * 32 + threadIdx.x;   // over [2][C]
   float s = 0.0f;
   if (i < 2 * g.C)
-    for (int n = threadIdx.y; n < g.N; n += 32) s += nc[(size_t)n * 2 * g.C + i];
+    for (int n = threadIdx.y; n < g.N; n += 32) s += __ldcg(nc + (size_t)n * 2 * g.C + i);
   sh[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && i < 2 * g.C) {
@@ -1253,6 +1259,7 @@ __global__ void __launch_bounds__(512, 1) gn_backward_slab_kernel(const void* __
       copy_commit();
     }
   }
+  ptx::grid_release();
   C cols;
   cols.set(g, b);
   f2 nmu[C::NP], rs[C::NP], ga[H], be[H];
@@ -1405,6 +1412,10 @@ struct GroupNormPlan : he_plan {
   }
 };
 
+// The folds start behind the kernel in front of them (launch_behind): a few small CTAs that are in place when its last one ends
+// (slabs backward [3,437,320] 9.2 -> 8.4 us, two passes backward [1,200000,77] 48.4 -> 45.2 us).  The second passes, and the
+// products of muon.cu, do not: started early, their many CTAs take the room of those still running (two passes forward
+// [2,262144,128] 84 -> 93 us, the conv net's filters 292 -> 299 us).
 template <int DT, int ACT, bool R>
 int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cudaStream_t st) {
   constexpr int V = Elem<DT>::V;
@@ -1438,8 +1449,8 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
     HE_CUDA(cudaLaunchKernelEx(&lc, kernel, in[0], in[1], out[0], (const float*)in[2], (const float*)in[3], (const float*)in[4],
                                (const float*)in[5], (float*)ws, g));
     const int param_ctas = (2 * g.C + 31) / 32;
-    gn_param_grads_kernel<<<param_ctas, dim3(32, 32), 0, st>>>((const float*)ws, (float*)out[1], (float*)out[2], nullptr, nullptr, g, param_ctas);
-    HE_CUDA(cudaGetLastError());
+    HE_TRY(launch_behind(gn_param_grads_kernel, dim3((unsigned)param_ctas), dim3(32, 32), 0, st, (const float*)ws, (float*)out[1], (float*)out[2],
+                         (const float*)nullptr, (float2*)nullptr, g, param_ctas));
     last_launches = 2;
     return HE_OK;
   }
@@ -1457,8 +1468,7 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
     HE_TRY(limits2[1].raise(gn_apply_kernel<DT, ACT, R>, ctx->device, kMaxSmem));
     gn_moments_kernel<DT, R><<<grid, threads, smem, st>>>(x, (float2*)ws, g);
     HE_CUDA(cudaGetLastError());
-    gn_fold_moments_kernel<<<g.N * g.G, 256, 0, st>>>((const float2*)ws, mean, rstd, g, slices, pitch);
-    HE_CUDA(cudaGetLastError());
+    HE_TRY(launch_behind(gn_fold_moments_kernel, dim3((unsigned)(g.N * g.G)), dim3(256), 0, st, (const float2*)ws, mean, rstd, g, slices, pitch));
     gn_apply_kernel<DT, ACT, R><<<grid, threads, ring, st>>>(x, out[0], gamma, beta, mean, rstd, g);
     HE_CUDA(cudaGetLastError());
     last_launches = 3;
@@ -1474,10 +1484,10 @@ int32_t GroupNormPlan::run(const void* const* in, void* const* out, void* ws, cu
   gn_grad_sums_kernel<DT, ACT, R><<<grid, threads, smem, st>>>(in[0], in[1], gamma, beta, mean, rstd, part, g);
   HE_CUDA(cudaGetLastError());
   const int param_ctas = (2 * g.C + 31) / 32, coef_ctas = (g.N * g.G + 31) / 32;
-  gn_fold_grads_kernel<<<dim3((unsigned)param_ctas, (unsigned)g.N), dim3(32, 32), 0, st>>>(part, nc, g, slices, g.nblk == 1 ? g.C : pitch);
-  HE_CUDA(cudaGetLastError());
-  gn_param_grads_kernel<<<param_ctas + coef_ctas, dim3(32, 32), 0, st>>>(nc, (float*)out[1], (float*)out[2], gamma, coef, g, param_ctas);
-  HE_CUDA(cudaGetLastError());
+  HE_TRY(launch_behind(gn_fold_grads_kernel, dim3((unsigned)param_ctas, (unsigned)g.N), dim3(32, 32), 0, st, (const float*)part, nc, g, slices,
+                       g.nblk == 1 ? g.C : pitch));
+  HE_TRY(launch_behind(gn_param_grads_kernel, dim3((unsigned)(param_ctas + coef_ctas)), dim3(32, 32), 0, st, (const float*)nc, (float*)out[1],
+                       (float*)out[2], gamma, coef, g, param_ctas));
   gn_grad_apply_kernel<DT, ACT, R><<<grid, threads, ring, st>>>(in[0], in[1], out[0], gamma, beta, mean, rstd, coef, g);
   HE_CUDA(cudaGetLastError());
   last_launches = 4;

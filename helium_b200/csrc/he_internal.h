@@ -123,6 +123,25 @@ class DeviceGuard {
   bool switched_ = false, failed_ = false;
 };
 
+// Launches a kernel that may start while the one before it in the stream drains (ptx::grid_wait in it says where it needs
+// what that one wrote).  Only for followers of this library's own kernels that call ptx::grid_release, in one he_launch; a
+// follower writes nothing in front of its grid_wait, and reads what the chain wrote behind it, through L2 (__ldcg).
+template <class... P, class... A>
+int32_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = block;
+  lc.dynamicSmemBytes = smem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = &attr;
+  lc.numAttrs = 1;
+  HE_CUDA(cudaLaunchKernelEx(&lc, kernel, static_cast<P>(args)...));
+  return HE_OK;
+}
+
 // Raises a kernel's limit of dynamic shared memory to all that an SM has, once on each device (the attribute belongs to
 // the function on the current device; a launch's own size decides occupancy).  One static object per kernel.
 class SmemLimit {

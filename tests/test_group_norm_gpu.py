@@ -343,3 +343,28 @@ def test_outputs_that_overlap_are_refused(ctx, p):
                  [torch.empty_like(x), v, v], [torch.empty_like(x), mean.view(c), vec()]):
         with pytest.raises(hb.HeliumError, match="overlaps"):
             bwd.launch([dy, x, gamma, beta, mean, rstd], outs)
+
+
+@pytest.mark.parametrize("size", [(3, 437, 320, 32), (1, 200000, 77, 7), (2, 33000, 64, 32), (2, 3, 2049, 3)])
+def test_chains_on_two_streams_at_once(ctx, size):
+    """Launches back to back on two streams, whose kernels overlap within a chain and between the streams: same bits each time."""
+    import torch
+    n, p, c, groups = size
+    fwd = hb.Plan.group_norm(ctx, "fwd", n, p, c, groups, activation="silu")
+    bwd = hb.Plan.group_norm(ctx, "bwd", n, p, c, groups, activation="silu")
+    sets, want = [], []
+    for seed in range(2):
+        x, gamma, beta, dy = _inputs(n, p, c, ir.BF16, seed)
+        y, mean, rstd = fwd.launch([x, gamma, beta])
+        sets.append((x, gamma, beta, dy, mean, rstd))
+        want.append([y, mean, rstd] + bwd.launch([dy, x, gamma, beta, mean, rstd]))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(20):
+        for k, (x, gamma, beta, dy, mean, rstd) in enumerate(sets):
+            with torch.cuda.stream(streams[k]):
+                got.append((k, fwd.launch([x, gamma, beta]) + bwd.launch([dy, x, gamma, beta, mean, rstd])))
+    torch.cuda.synchronize()
+    for k, outs in got:
+        for a, b in zip(outs, want[k]):
+            assert torch.equal(a, b)
