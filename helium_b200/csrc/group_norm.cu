@@ -1572,8 +1572,8 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
   // estimated from what was measured on a B200: a CTA's life is a fixed part (issue, folds, exchange: 4 us, with a
   // cluster 1.5 us more) and a part for each of its vectors; shared memory says how many live on an SM at once, gangs of
   // CTAs fill it to some 85 %; an SM issues 18 (backward 40) instructions a value; row segments below 64 bytes waste half
-  // of DRAM's sectors.  ([64,3136,256] bf16 silu forward: 64-byte segments in clusters of 8 x 128 threads 52 us, 512-byte
-  // ones in clusters of 8 x 512 threads 98 us; [128,784,128] backward: 33 us and 47 us.)
+  // of DRAM's sectors.  ([64,3136,256] bf16 silu forward: 64-byte segments in clusters of 8 x 128 threads 50 us, 512-byte
+  // ones in clusters of 8 x 512 threads 98 us; [128,784,128] backward: 32 us and 47 us.)
   const long long srows = ((long long)g.P + g.f - 1) / g.f + (plan->ragged ? 1 : 0);
   const bool fwd = direction == HE_GN_FORWARD;
   const int es = dtype_bytes(prm->dtype);
@@ -1611,8 +1611,8 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
     }
   }
   // Against two passes over all of it (three launches forward, four backward, 5.6 TB/s): worth it for the largest tensors
-  // only, where the slabs' folds and exchanges add up ([64,3136,256] bf16: backward 105 us in two passes, 129 us in slabs,
-  // forward 73 and 52 us; [128,784,128] backward 41 and 33 us).
+  // only, where the slabs' folds and exchanges add up ([64,3136,256] bf16: backward 102 us in two passes, 129 us in slabs,
+  // forward 73 and 50 us; [128,784,128] backward 41 and 32 us).
   const double two_us = (fwd ? 18.0 : 22.0) + (double)g.total * es * (fwd ? 3 : 5) / 5.6e6;
   if (plan->cluster && 6.0 + 1.25 * best > two_us) plan->cluster = 0;
   if (plan->cluster) {
