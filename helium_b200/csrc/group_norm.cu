@@ -16,8 +16,8 @@
 //
 // Sums are f32.  The forward moments are taken about a shift: in the two-pass kernels one of each thread's own (the first
 // value it sees), whose sums become the thread's about the group mean m by q - 2 d s + n d^2 with d = m - shift; in the slab
-// kernels the group's first value, and where that lies far from the mean a second round over the tile, which is on chip,
-// takes the mean instead.  Either way the cancellation is bounded whatever the tensor's mean is.  Every fold runs in a fixed
+// kernels the group's first value, and where that (or zero) lies far from the mean a second round over the tile, which is on
+// chip, takes the mean instead.  Either way the cancellation is bounded whatever the tensor's mean is.  Every fold runs in a fixed
 // order: results repeat bit for bit.
 #include <algorithm>
 #include <cmath>
@@ -1010,8 +1010,9 @@ template <int R, int V> __device__ __forceinline__ void fold_groups(const GnGeom
   }
 }
 
-// Sums of x - shift and of its square.  The shift of a group is one of its values, the picture's first: all CTAs of the
-// cluster take the same one, so their sums simply add up.
+// Sums of x and of (x - shift)^2.  The shift of a group is one of its values, the picture's first: all CTAs of the cluster
+// take the same one, so their sums simply add up.  x itself is added, not x - shift, whose mean would carry the rounding of
+// |mean - shift| where the mean is next to nothing.  The second round, whose shift is the mean, adds x - shift (kAbout).
 template <int DT, int R> struct ShiftedSums {
   static constexpr int V = Elem<DT>::V, H = V / 2;
   typedef Cols<V, R> C;
@@ -1020,25 +1021,27 @@ template <int DT, int R> struct ShiftedSums {
 #pragma unroll
     for (int h = 0; h < H; ++h) s[h] = q[h] = pk(0.0f, 0.0f);
   }
-  __device__ __forceinline__ void add(const uint4& v) {
+  template <bool kAbout> __device__ __forceinline__ void add(const uint4& v) {
     f2 x[H];
     Elem<DT>::unpack(v, x);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const f2 d = add2(x[h], nshift[C::pair(h)]);
-      s[h] = add2(s[h], d);
+      s[h] = add2(s[h], kAbout ? d : x[h]);
       q[h] = fma2(d, d, q[h]);
     }
   }
-  __device__ void add_edge(const uint4& v, long long e, long long lo, long long hi) {
+  template <bool kAbout> __device__ void add_edge(const uint4& v, long long e, long long lo, long long hi) {
     f2 x[H];
     Elem<DT>::unpack(v, x);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      float da, db;
+      const bool ia = e + 2 * h >= lo && e + 2 * h < hi, ib = e + 2 * h + 1 >= lo && e + 2 * h + 1 < hi;
+      float xa, xb, da, db;
+      un(x[h], xa, xb);
       un(add2(x[h], nshift[C::pair(h)]), da, db);
-      const f2 d = pk(e + 2 * h >= lo && e + 2 * h < hi ? da : 0.0f, e + 2 * h + 1 >= lo && e + 2 * h + 1 < hi ? db : 0.0f);
-      s[h] = add2(s[h], d);
+      const f2 d = pk(ia ? da : 0.0f, ib ? db : 0.0f);
+      s[h] = add2(s[h], kAbout ? d : pk(ia ? xa : 0.0f, ib ? xb : 0.0f));
       q[h] = fma2(d, d, q[h]);
     }
   }
@@ -1093,7 +1096,7 @@ __global__ void __launch_bounds__(512, 2) gn_forward_slab_kernel(const void* __r
         const long long e = row * g.W + (long long)b.vcol * V;
         const uint4 v = load_edge<DT>(x, e, g.total);
         tile[(size_t)(row - h.s0) * g.cols + b.j] = v;
-        m.add_edge(v, e, h.lo, h.hi);
+        m.template add_edge<false>(v, e, h.lo, h.hi);
       });
   }
   {
@@ -1104,12 +1107,14 @@ __global__ void __launch_bounds__(512, 2) gn_forward_slab_kernel(const void* __r
       copy_wait(kPieces - k);
       const int end = min(b.rows, k * b.piece);
 #pragma unroll 2
-      for (; r < end; r += g.lanes, src += tstep) m.add(*src);
+      for (; r < end; r += g.lanes, src += tstep) m.template add<false>(*src);
     }
   }
-  // Totals of the cluster, and the variance from them.  Where the shift turns out to be far from the mean (16 times the
-  // variance), the squares have cancelled too much: then a second round over the tile takes the mean as its shift.
-  // Every CTA of the cluster sees the same totals, so they agree on it.
+  // Totals of the cluster, and the variance from them.  Where the shift turns out to be far from the mean (its square 16 times
+  // the variance) the squares have cancelled too much, and where the mean is far from zero (16 times as well) its rounding
+  // is too much for the variance: then a second round over the tile takes the mean as its shift.  Every CTA of the cluster
+  // sees the same totals, so they agree on it.
+  const float count = (float)g.P * (float)g.cpg;
   for (int round = 0; round < 2; ++round) {
     float* sums = round ? own2 : own;
     fold_groups<R, V>(g, b, m.s, m.q, red, part, sums);
@@ -1132,11 +1137,11 @@ __global__ void __launch_bounds__(512, 2) gn_forward_slab_kernel(const void* __r
         tq = sums[b.groups + k];
       }
       const float shift = round ? mean_s[k] : load_param_as_f32(x, DT, corner + k * g.cpg);
-      const float d = ts * g.inv_count, sq = fmaf(-d, ts, tq);
-      const float mean = shift + d, rstd = 1.0f / sqrtf((sq < 0.0f ? 0.0f : sq) * g.inv_count + g.eps);
+      const float of_sum = ts * g.inv_count, mean = round ? shift + of_sum : of_sum, d = round ? of_sum : of_sum - shift;
+      const float sq = fmaf(-d * count, d, tq), rstd = 1.0f / sqrtf((sq < 0.0f ? 0.0f : sq) * g.inv_count + g.eps);
       mean_s[k] = mean;
       rstd_s[k] = rstd;
-      const bool more = round == 0 && sq * 16.0f < tq;
+      const bool more = round == 0 && (sq * 16.0f < tq || mean * mean * count > 16.0f * sq);
       again = again || more;
       if (b.rank == 0) {   // written again by a second round
         const size_t out = (size_t)b.n * g.G + (size_t)b.blk * b.groups + k;
@@ -1150,10 +1155,10 @@ __global__ void __launch_bounds__(512, 2) gn_forward_slab_kernel(const void* __r
     if (b.active) {
       cols.by_group(m.nshift, [&](int k) { return -mean_s[k]; });
       const uint4* src = mine;
-      for (int r = 0; r < b.rows; r += g.lanes, src += tstep) m.add(*src);
+      for (int r = 0; r < b.rows; r += g.lanes, src += tstep) m.template add<true>(*src);
       if (kRagged)
         edge_rows(g, h, b.lane, [&](long long row) {
-          m.add_edge(tile[(size_t)(row - h.s0) * g.cols + b.j], row * g.W + (long long)b.vcol * V, h.lo, h.hi);
+          m.template add_edge<true>(tile[(size_t)(row - h.s0) * g.cols + b.j], row * g.W + (long long)b.vcol * V, h.lo, h.hi);
         });
     }
   }
