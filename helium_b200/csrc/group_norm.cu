@@ -1111,9 +1111,10 @@ __global__ void __launch_bounds__(512, 2) gn_forward_slab_kernel(const void* __r
     }
   }
   // Totals of the cluster, and the variance from them.  Where the shift turns out to be far from the mean (its square 16 times
-  // the variance) the squares have cancelled too much, and where the mean is far from zero (16 times as well) its rounding
-  // is too much for the variance: then a second round over the tile takes the mean as its shift.  Every CTA of the cluster
-  // sees the same totals, so they agree on it.
+  // the variance) the squares have cancelled too much, and where the mean is as far from zero its rounding is too much for
+  // the variance: then a second round over the tile takes the mean as its shift.  (By the root-mean-square and the largest
+  // error of rstd in half steps of f32: mean at 4 deviations 3.7 and 20, at 7 5.9 and 48, after a second round 0.8 and 2.4.
+  // It takes [64,3136,256] from 50 to 65 us.)  Every CTA of the cluster sees the same totals, so they agree on it.
   const float count = (float)g.P * (float)g.cpg;
   for (int round = 0; round < 2; ++round) {
     float* sums = round ? own2 : own;
