@@ -118,14 +118,21 @@ __device__ __forceinline__ f2 reciprocals(f2 v) {
   return pk(rcp(a), rcp(b));
 }
 // 1 / (1 + exp(-z)).  One reciprocal serves a pair, b / (a b) and a / (a b): the special-function unit, 8 cycles a warp, is all
-// but the bound here (two passes backward over a [2,512,512,128] tensor: 128 -> 121 us).  exp is held at 2^63 (z = -43.7) so
-// that the product is finite: below it the result is 1e-19.  (GELU, which waits for other things, was 2 % slower that way.)
+// but the bound here (two passes backward over a [2,512,512,128] tensor: 128 -> 121 us).  a = 2^-63 (1 + exp(-z)) with exp held
+// at 2^126.4, so that a lies between 2^-63 and 2^63.4 and the product and its reciprocal in f32's range; the sigmoid is right down
+// to 2^-126 and below that flushed to zero (z < -87.6; a NaN's too, z times which is a NaN again).  (A branch to two reciprocals
+// where a product of unscaled terms overflows: 50.2 -> 56.4 us for [64,3136,256] bf16 forward.  GELU, which waits for other
+// things, was 2 % slower with one.)
 __device__ __forceinline__ f2 sigmoid2(f2 z) {
+  const f2 scale = pk(1.0842021724855044e-19f, 1.0842021724855044e-19f);   // 2^-63
   float a, b;
   un(mul2(z, pk(-1.4426950408889634f, -1.4426950408889634f)), a, b);
-  un(add2(pk(ex2(fminf(a, 63.0f)), ex2(fminf(b, 63.0f))), pk(1.0f, 1.0f)), a, b);
+  un(fma2(pk(ex2(fminf(a, 126.4f)), ex2(fminf(b, 126.4f))), scale, scale), a, b);
   const float r = rcp(a * b);
-  return mul2(pk(b, a), pk(r, r));
+  const f2 v = mul2(pk(b, a), pk(r, r));
+  f2 s;
+  asm("mul.rn.ftz.f32x2 %0, %1, %2;" : "=l"(s) : "l"(v), "l"(scale));
+  return s;
 }
 // Normal cumulative distribution, and exp(-z^2 / 2) beside it: half of erfc(|z| / sqrt 2) on the negative side (no
 // cancellation in the tail), one minus that on the other.  f32 tensors take the Chebyshev form of Numerical Recipes
