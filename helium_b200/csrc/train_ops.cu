@@ -286,13 +286,11 @@ __global__ void __launch_bounds__(256) colsum_bf16_kernel(const uint4* __restric
 }
 
 // SGD with helium's momentum: avg = first ? g : g (1 - m) + avg m;  w -= lr avg;  w16 = bf16(w)
-template <typename G>
-__global__ void __launch_bounds__(256) sgd_momentum_kernel(float* __restrict__ w, float* __restrict__ avg, const G* __restrict__ g,
+template <int DT>
+__global__ void __launch_bounds__(256) sgd_momentum_kernel(float* __restrict__ w, float* __restrict__ avg, const void* __restrict__ g,
                                                            unsigned short* __restrict__ w16, long long n, float lr, float m, int first) {
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-    float gv;
-    if (sizeof(G) == 4) gv = reinterpret_cast<const float*>(g)[i];
-    else gv = bf16_bits_to_f32(reinterpret_cast<const unsigned short*>(g)[i]);
+    const float gv = load_param_as_f32(g, DT, i);
     const float a = first || !avg ? gv : gv * (1.0f - m) + avg[i] * m;   // no average: plain SGD
     if (avg) avg[i] = a;
     const float nw = w[i] - a * lr;
@@ -564,15 +562,12 @@ int32_t he_colsum_bf16(const void* x, float* out, void* workspace, int64_t pixel
 int32_t he_sgd_momentum(float* w, float* avg, const void* grad, int32_t grad_dtype, void* w_bf16, int64_t n, float lr, float momentum,
                         int32_t first_step, void* cu_stream) {
   if (!w || !grad || n <= 0) HE_FAIL(HE_ERR_INVALID, "he_sgd_momentum: bad argument");
-  if (grad_dtype != HE_F32 && grad_dtype != HE_BF16) HE_FAIL(HE_ERR_UNSUPPORTED, "he_sgd_momentum: gradients must be f32 or bf16");
+  if (grad_dtype != HE_F32 && grad_dtype != HE_BF16 && grad_dtype != HE_F16)
+    HE_FAIL(HE_ERR_UNSUPPORTED, "he_sgd_momentum: gradients must be f32, bf16 or f16");
   const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 148 * 16);
   cudaStream_t st = (cudaStream_t)cu_stream;
-  if (grad_dtype == HE_F32)
-    sgd_momentum_kernel<float><<<grid, 256, 0, st>>>(w, avg, reinterpret_cast<const float*>(grad), reinterpret_cast<unsigned short*>(w_bf16), n, lr,
-                                                     momentum, first_step);
-  else
-    sgd_momentum_kernel<unsigned short><<<grid, 256, 0, st>>>(w, avg, reinterpret_cast<const unsigned short*>(grad),
-                                                              reinterpret_cast<unsigned short*>(w_bf16), n, lr, momentum, first_step);
+  auto kernel = grad_dtype == HE_F32 ? sgd_momentum_kernel<HE_F32> : grad_dtype == HE_BF16 ? sgd_momentum_kernel<HE_BF16> : sgd_momentum_kernel<HE_F16>;
+  kernel<<<grid, 256, 0, st>>>(w, avg, grad, reinterpret_cast<unsigned short*>(w_bf16), n, lr, momentum, first_step);
   HE_CUDA(cudaGetLastError());
   return HE_OK;
 }

@@ -408,7 +408,8 @@ int32_t he_add_bf16(const void* a, const void* b, void* out, int64_t n, void* cu
 int32_t he_colsum_bf16(const void* x, float* out, void* workspace, int64_t pixels, int32_t channels, void* cu_stream);
 /* Sgd::step with momentum (helium/src/optimizer/sgd.rs:47-62): avg = first_step ? g : g (1 - m) + avg m;
  * w -= lr * avg; `w_bf16` (may be NULL) receives the updated weights rounded to bf16, the copy the next
- * step's convolutions read (helium/src/modules/conv.rs:63).  `avg` may be NULL for plain SGD (momentum 0). */
+ * step's convolutions read (helium/src/modules/conv.rs:63).  `avg` may be NULL for plain SGD (momentum 0).  `grad` is F32, BF16
+ * or F16. */
 int32_t he_sgd_momentum(float* w, float* avg, const void* grad, int32_t grad_dtype, void* w_bf16, int64_t n, float lr,
                         float momentum, int32_t first_step, void* cu_stream);
 /* The Muon optimiser's update for a list of weight matrices: each gradient's momentum average, orthogonalised by
