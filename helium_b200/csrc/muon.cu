@@ -179,6 +179,15 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// The factor sx / (|d| + eps) of the direction as two, `pre` a power of two: for |d| + eps below 1e-34 it leaves f32's range
+// (denormal gradients, or a zero one with a tiny eps, which has to come out as zero).  pre d is at most 2^15 there.
+__device__ __forceinline__ float direction_scale(double sum_of_squares, float sx, float eps, float& pre) {
+  const double f = (double)sx / (sqrt(sum_of_squares) + (double)eps);
+  const bool far = f > 0x1p96;
+  pre = far ? 0x1p96f : 1.0f;
+  return (float)(far ? f * 0x1p-96 : f);
+}
+
 // ---- second pass: the direction, scaled and split, into the blocks of the workspace; zeros behind its edges ----------
 // A CTA fills one block of 128 rows x 64 columns.  Where the gradient's rows run along X's and are whole vectors a thread
 // reads 8 columns and writes them; otherwise the block goes through shared memory, read along the gradient's own rows.
@@ -250,7 +259,8 @@ __global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ 
   }
   __syncthreads();
   s = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
-  const float scale = (float)((double)m.sx / (sqrt(s) + (double)st.eps));
+  float pre;
+  const float scale = direction_scale(s, m.sx, st.eps, pre);
 #pragma unroll
   for (int i = 0; i < kBlockRows * 8 / 256; ++i) {
     const int r = (threadIdx.x >> 3) + 32 * i, q = (threadIdx.x & 7) * 8;
@@ -263,7 +273,7 @@ __global__ void __launch_bounds__(256) muon_pack_kernel(const __grid_constant__ 
     }
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair(v[2 * j] * scale, v[2 * j + 1] * scale, hi[j], lo[j]);
+    for (int j = 0; j < 4; ++j) split_pair(v[2 * j] * pre * scale, v[2 * j + 1] * pre * scale, hi[j], lo[j]);
     *reinterpret_cast<uint4*>(hi_at + r * 128 + q * 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(lo_at + r * 128 + q * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
@@ -1022,7 +1032,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) muon_small_kernel(const __gr
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
   sum = 0.0;
   for (int i = 0; i < kSmallThreads / 32; ++i) sum += sh.sums[i];
-  const float scale = (float)((double)m.sx / (sqrt(sum) + (double)st.eps));
+  float pre;
+  const float scale = direction_scale(sum, m.sx, st.eps, pre);
   // scaled and split into the blocks
   {
     float v[kSmallBlocks][16];
@@ -1040,7 +1051,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) muon_small_kernel(const __gr
       if (b < blocks) {
         uint32_t hi[8], lo[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) split_pair(v[b][2 * q] * scale, v[b][2 * q + 1] * scale, hi[q], lo[q]);
+        for (int q = 0; q < 8; ++q) split_pair(v[b][2 * q] * pre * scale, v[b][2 * q + 1] * pre * scale, hi[q], lo[q]);
         store_block_row(smem + b * kOperandBytes, r, team * 16, hi);
         store_block_row(smem + kOffSmallLo + b * kOperandBytes, r, team * 16, lo);
       }
