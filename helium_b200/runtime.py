@@ -36,6 +36,13 @@ def _cuda_device(torch, index: int):
     return d
 
 
+def _int(what: str, v: int, bits: int = 32) -> int:
+    """`v`, if it fits the C field it goes into (ctypes drops the bits that do not)."""
+    if not -(1 << (bits - 1)) <= v < 1 << (bits - 1):
+        raise ValueError(f"{what} {v} does not fit {bits} bits")
+    return v
+
+
 def _checked_ptr(t, spec, dev: int, what: str, i: int) -> int:
     """Address of a dense tensor of the shape and type that the plan wants there, on the plan's device."""
     if t.shape != spec[0] or t.dtype is not spec[1]:
@@ -173,7 +180,8 @@ class Plan:
         gamma, beta; outputs y, mean, rstd) or "bwd" (inputs dy, x, gamma, beta, mean, rstd; outputs dx, dgamma, dbeta).
         activation: "none", "relu", "silu" or "gelu"."""
         d = {"fwd": 0, "bwd": 1}[direction]
-        prm = HeGroupNormParams(batch, channels, positions, groups, dtype, {"none": 0, "relu": 1, "silu": 2, "gelu": 3}[activation], eps)
+        prm = HeGroupNormParams(_int("batch", batch), _int("channels", channels), _int("positions", positions, 64), _int("groups", groups),
+                                _int("dtype", dtype), {"none": 0, "relu": 1, "silu": 2, "gelu": 3}[activation], eps)
         h = C.c_void_p()
         check(lib.he_plan_group_norm(ctx._h if ctx else None, d, C.byref(prm), C.byref(h)))
         x = (batch, positions, channels)
@@ -193,13 +201,18 @@ class Plan:
         """he_plan_muon for matrices of `shapes` [(rows, cols), ...].  Inputs: the gradients, then (unless `momentum` is
         None) the f32 averages; outputs: the updates, then the new averages, which may be written over the old ones."""
         n = len(shapes)
-        rows = (C.c_int64 * max(1, n))(*[s[0] for s in shapes])
-        cols = (C.c_int64 * max(1, n))(*[s[1] for s in shapes])
+        for s in shapes:
+            if len(s) != 2:
+                raise ValueError(f"a matrix has two sizes, got {tuple(s)}")
+        if len(coefs) != 3:
+            raise ValueError(f"coefs are a, b, c, got {len(coefs)} numbers")
+        rows = (C.c_int64 * max(1, n))(*[_int("rows", s[0], 64) for s in shapes])
+        cols = (C.c_int64 * max(1, n))(*[_int("cols", s[1], 64) for s in shapes])
         if scales is not None and len(scales) != n:
             raise ValueError(f"{n} matrices, {len(scales)} scales")
         sc = (C.c_float * max(1, n))(*scales) if scales is not None else None
         m = 0.0 if momentum is None else momentum
-        prm = HeMuonParams(n, rows, cols, sc, grad_dtype, out_dtype, steps, (C.c_float * 3)(*coefs), eps, int(momentum is not None), m,
+        prm = HeMuonParams(n, rows, cols, sc, _int("grad_dtype", grad_dtype), _int("out_dtype", out_dtype), _int("steps", steps), (C.c_float * 3)(*coefs), eps, int(momentum is not None), m,
                            int(nesterov))
         h = C.c_void_p()
         check(lib.he_plan_muon(ctx._h if ctx else None, C.byref(prm), C.byref(h)))
