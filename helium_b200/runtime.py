@@ -285,7 +285,8 @@ class Plan:
         """`launch` of the plans that know their operands' shapes: every tensor is checked, the stream is the current one
         of the plan's device, and the workspace belongs to this launch alone (taken from torch's allocator on the launching
         stream: part of the graph's pool under capture), so launches on several streams and several captured graphs never
-        share one."""
+        share one.  With another `stream` the allocator is told that it uses the tensors, and the current one the new outputs:
+        memory of either that is let go is not handed out again before both are through."""
         if self._torch_specs is None:
             as_torch = lambda spec: (tuple(spec[0]), _TORCH_DTYPES[spec[1]])  # noqa: E731
             in_specs = [as_torch(spec) for spec in self._in_specs]
@@ -298,11 +299,23 @@ class Plan:
                                  C.c_void_p * len(in_specs), C.c_void_p * len(out_specs))
         in_specs = self._torch_specs[0]
         dev = self.ctx.device if self.ctx else 0
-        ins = [_checked_ptr(t, spec, dev, "input", i) for i, (t, spec) in enumerate(zip(inputs, in_specs))]
+        target = stream
         if stream is not None:
-            target = torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream
+            if isinstance(stream, int):
+                target = torch.cuda.ExternalStream(stream, device=dev)
+            if target.device.index != dev:
+                raise ValueError(f"the stream is on {target.device}, the plan on cuda:{dev}")
+        ins = [_checked_ptr(t, spec, dev, "input", i) for i, (t, spec) in enumerate(zip(inputs, in_specs))]
+        if target is not None:
+            current, made = torch.cuda.current_stream(dev), outputs is None
             with torch.cuda.stream(target):
-                return self._launch_on(torch, target.cuda_stream, dev, inputs, ins, outputs)
+                outputs = self._launch_on(torch, target.cuda_stream, dev, inputs, ins, outputs)
+            if target.cuda_stream != current.cuda_stream:
+                for t in inputs:
+                    t.record_stream(target)
+                for t in outputs:
+                    t.record_stream(current if made else target)
+            return outputs
         return self._launch_on(torch, torch._C._cuda_getCurrentRawStream(dev), dev, inputs, ins, outputs)
 
     def _launch_on(self, torch, stream_ptr, dev, inputs, ins, outputs):

@@ -35,3 +35,15 @@ def test_muon_takes_matrices(shape):
     """A filter is given as its K x RSC matrix: of [K, R, S, C] the first two sizes alone would be another matrix."""
     with pytest.raises(ValueError, match="two sizes"):
         hb.Plan.muon(None, [(8, 8), shape])
+
+
+def test_a_stream_of_another_device_is_refused():
+    import torch
+
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 0
+
+    plan = hb.Plan.group_norm(None, "fwd", 1, 9, 16, 4)
+    x = torch.zeros(1, 9, 16, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        plan.launch([x, torch.zeros(16), torch.zeros(16)], stream=Stream())
