@@ -14,35 +14,20 @@
 
 #include "gemm_plan.cuh"
 #include "pointwise_dense.cuh"
+#include "tensor_map.h"
 
 namespace he {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
-// TMA descriptor encoding through the driver entry point (no link-time dependency on libcuda)
+// TMA descriptors
 // ------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
 
 // Operand tensor [batch, R, K] (K-major) or [batch, K, R] (MN-major), 2-byte elements.
 // `pitch` = elements between consecutive rows of the stored matrix (0: dense, i.e. K or R).
 int32_t make_operand_tmap(CUtensorMap* out, const void* ptr, int ab_format, bool mn_major, int64_t R, int64_t K,
                           int64_t batch, int box_rows, int64_t pitch = 0) {
-  EncodeTiledFn fn = get_encode_fn();
+  EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) HE_FAIL(HE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   if ((uintptr_t)ptr % 16 != 0) HE_FAIL(HE_ERR_UNSUPPORTED, "fused matmul: operand pointer is not 16-byte aligned");
   cuuint64_t dims[3], strides[2];
@@ -68,7 +53,7 @@ int32_t make_operand_tmap(CUtensorMap* out, const void* ptr, int ab_format, bool
 
 // 8-bit operand copy [batch, R, k_pitch] bytes, K-major: box = 128 bytes of K x box_rows rows.
 int32_t make_f8_tmap(CUtensorMap* out, const void* ptr, int64_t R, int64_t K, int64_t k_pitch, int64_t batch, int box_rows) {
-  EncodeTiledFn fn = get_encode_fn();
+  EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) HE_FAIL(HE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)R, (cuuint64_t)batch};
   cuuint64_t strides[2] = {(cuuint64_t)k_pitch, (cuuint64_t)R * k_pitch};

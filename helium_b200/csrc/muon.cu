@@ -28,6 +28,7 @@
 #include "device_utils.cuh"
 #include "he_internal.h"
 #include "gemm_sm100_2cta.cuh"
+#include "tensor_map.h"
 
 namespace he {
 namespace {
@@ -1222,21 +1223,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) muon_small_kernel(const __gr
 }
 
 // ---- plan --------------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                  CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
 int32_t encode_arena(CUtensorMap* map, void* arena, long long rows, int box_rows) {
-  EncodeTiledFn fn = encode_fn();
+  EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) HE_FAIL(HE_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t dims[3] = {kBlockCols, (cuuint64_t)rows, 1};
   const cuuint64_t strides[2] = {128, (cuuint64_t)rows * 128};
