@@ -704,7 +704,8 @@ __global__ void __launch_bounds__(512, 1) gn_apply_kernel(const void* __restrict
   constexpr int V = Elem<DT>::V, H = V / 2;
   const int n = blockIdx.z, vcol = blockIdx.y * g.cols + threadIdx.x % g.cols, lane = threadIdx.x / g.cols;
   if (lane >= g.lanes || vcol * V >= g.W) return;
-  // slices are walked from the last one down: the moments pass ended there, so their values are the likeliest in L2
+  // a picture's slices are taken from the last one down: with one picture the moments pass ended there, so its values are the
+  // likeliest in L2 (with several it ended in the last picture, and this pass begins with the first: no reuse is counted on)
   const Share h = share_of(g, n, gridDim.x - 1 - blockIdx.x);
   int c[V];
   thread_channels<V>(g, vcol, c);
@@ -1647,7 +1648,10 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
   }
   // Against two passes over all of it (three launches forward, four backward, 5.6 TB/s): worth it for the largest tensors
   // only, where the slabs' folds and exchanges add up ([64,3136,256] bf16: backward 102 us in two passes, 129 us in slabs,
-  // forward 73 and 50 us; [128,784,128] backward 41 and 32 us).
+  // forward 73 and 50 us; [128,784,128] backward 41 and 32 us).  The constants were fitted to 16-bit types.  f32 backward, slabs and
+  // two passes: [128,784,128] 44 and 54 us, [128,196,256] 21 and 34, [16,1024,320] 25 and 27 -- and five shapes where the estimate
+  // takes slabs and two passes are the faster: [64,3136,256] 204 and 183 us, [128,3136,64] 105 and 95, [32,3136,64] 31 and 28,
+  // [4,4096,512] 36 and 33, [8,4096,128] 23 and 20.  bf16 has one such, [32,3136,64] backward, 28 and 26 us; forward has none.
   const double two_us = (fwd ? 18.0 : 22.0) + (double)g.total * es * (fwd ? 3 : 5) / 5.6e6;
   if (plan->cluster && 6.0 + 1.25 * best > two_us) plan->cluster = 0;
   if (plan->cluster) {
@@ -1665,8 +1669,10 @@ int32_t plan_group_norm(he_ctx* ctx, int32_t direction, const he_group_norm_para
   g.cols = std::min(vcols, plan->threads);
   g.nblk = (vcols + g.cols - 1) / g.cols;
   g.lanes = plan->threads / g.cols;
-  // slices: what lives on the SMs at once (shared memory holds the rings of 6 CTAs forward, 3 backward), at least 16
-  // super-rows a thread (the folds' cost is per CTA)
+  // slices: as many CTAs as shared memory has rings for, 6 an SM forward and 3 backward of 256 threads, and at least 16 super-rows
+  // a thread (the folds' cost is per CTA).  Registers let fewer live: 3 of the moments pass (80), 2 or 3 of the others (16-bit types:
+  // gn_apply_kernel 72-96, gn_grad_sums_kernel 78-126, gn_grad_apply_kernel 94-126), so a grid is two or three waves forward and one
+  // and a half backward.
   const long long per_min = (long long)g.lanes * 16;
   long long want = std::max<long long>(1, (long long)sms * (fwd ? 6 : 3) * 256 / plan->threads / std::max<long long>(1, (long long)g.N * g.nblk));
   want = std::min(want, std::max<long long>(1, srows / per_min));

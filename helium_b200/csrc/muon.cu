@@ -14,8 +14,9 @@
 // when a call is planned), S by 2^12, B by 2^10.  X itself is kept as a pair hi + lo of f16 (22 bits): the products read
 // hi, the term a X adds the pair, so the rounding of hi is not multiplied by a = 3.4 step after step, and B's diagonal, by
 // far its largest values, stays f32 and is applied to the pair too.
-// Simulated against 64 bits, the update is 4e-4 .. 9e-4 off (relative, 2-norm), half a bf16 rounding of the result;
-// bf16 operands were 4e-3 .. 2e-2 off, f16 without the pair 2e-3 .. 5e-3.
+// Measured against 64 bits (f16 updates, their own rounding taken out), an update is 3e-4 .. 1.1e-3 off (relative, 2-norm):
+// 32 x 152 and 64 x 32 filters 1.1e-3, 64 x 576 6.8e-4, 512 x 2304 6.4e-4, 4096 x 4096 6.0e-4; a bf16 update's rounding alone is
+// 1.7e-3.  In a simulation bf16 operands were 4e-3 .. 2e-2 off, f16 without the pair 2e-3 .. 5e-3.
 //
 // Layout.  The workspace holds every matrix as blocks of 128 rows x 64 columns, 128 bytes a row, block after block: one
 // tensor map over the whole workspace serves all operands of all matrices, whatever their shapes.  A block is a K-major
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(kSumThreads, 8) muon_average_kernel(const __gr
   const long long total = (long long)m.m * m.n;
   const long long e0 = (long long)(blockIdx.x - m.part0) * m.chunk, e1 = min(total, e0 + m.chunk);
   double sum = 0.0;
-  constexpr int U = 2;     // vectors of 4 elements a thread keeps in flight (conv net's filters: 1 293 us, 2 291 us, 4 299 us)
+  constexpr int U = 2;     // vectors of 4 elements a thread keeps in flight (conv net's filters: 4 299 us; 1 and 2, 293 and 291 us, are within 1 %)
   for (long long e = e0 + threadIdx.x * 4; e < e1; e += U * kSumThreads * 4) {
     float g[U][4], av[U][4];
 #pragma unroll
@@ -1409,7 +1410,9 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     r.table.count = std::min(kMaxMats, prm->count - first);
     r.index.assign(order.begin() + first, order.begin() + first + r.table.count);
     const int sms = ctx_sm_count(ctx);
-    // Every matrix of this part of the list fits an SM (where only some do, the others' tiles leave room for theirs)
+    // Every matrix of this part of the list fits an SM.  Where only some do, all go by tiles: the small ones' tiles find room
+    // beside the others' (32 of 64 x 288 with one 64 x 576 100 us in one list, 139 us in two, 43 of them the small ones' kernel; 40 of
+    // them with one 512 x 4608 177 and 213 us).
     r.small = true;
     for (int i = 0; i < r.table.count; ++i) {
       const int64_t h = prm->rows[r.index[i]], w = prm->cols[r.index[i]];
@@ -1418,7 +1421,8 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
     // Which tiles: a phase lasts as long as its deepest tile and a fixed part (waits, first loads, epilogue), or as its
     // whole work spread over the workers, if that is longer.  Measured on a B200: 0.35 us a 64-deep block and 5 us fixed for
     // 128 x 128 tiles, 0.41 us and 8 us for 256 x 256 tiles of a pair.  (A 1024 x 1024 matrix takes 166 us on single CTAs and
-    // 222 us on pairs, 2048 x 8192 851 and 767, 4096 x 4096 1790 and 1257.)
+    // 222 us on pairs, 2048 x 8192 851 and 767, 4096 x 4096 1790 and 1257.)  One size for the whole list: 4096 x 4096 with 16 of
+    // 512 x 512 takes 1307 us so, in two lists with a size each 1450 us; with the conv net's filters 1449 and 1588 us.
     long long s_blocks1 = 0, s_blocks2 = 0;
     for (int i = 0; i < r.table.count; ++i) {
       const int64_t h = prm->rows[r.index[i]], w = prm->cols[r.index[i]];
@@ -1476,7 +1480,7 @@ int32_t plan_muon(he_ctx* ctx, const he_muon_params* prm, he_plan** out) {
       m.b0 = (int)items_b; items_b += tiles;
       m.x0 = (int)items_x; items_x += ti * tj;
       m.pack0 = (int)pack; pack += (long long)m.mt * 2 * m.nt;
-      // partial sums: CTAs of at least 4096 elements, at most 2048 of them (4096 x 4096: 512 of them 1228 us, 2048 1218 us)
+      // partial sums: CTAs of at least 4096 elements, at most 2048 of them (512 or 2048 are within 1 % for 4096 x 4096)
       const long long total = (long long)m.m * m.n;
       long long chunks = std::min<long long>(2048, (total + 4095) / 4096);
       m.chunk = (total + chunks - 1) / chunks;
