@@ -14,9 +14,9 @@
 // when a call is planned), S by 2^12, B by 2^10.  X itself is kept as a pair hi + lo of f16 (22 bits): the products read
 // hi, the term a X adds the pair, so the rounding of hi is not multiplied by a = 3.4 step after step, and B's diagonal, by
 // far its largest values, stays f32 and is applied to the pair too.
-// Measured against 64 bits (f16 updates, their own rounding taken out), an update is 3e-4 .. 1.1e-3 off (relative, 2-norm):
-// 32 x 152 and 64 x 32 filters 1.1e-3, 64 x 576 6.8e-4, 512 x 2304 6.4e-4, 4096 x 4096 6.0e-4; a bf16 update's rounding alone is
-// 1.7e-3.  In a simulation bf16 operands were 4e-3 .. 2e-2 off, f16 without the pair 2e-3 .. 5e-3.
+// Measured against 64 bits (the update's own rounding taken out), an update of five steps is 3e-4 .. 1.1e-3 off (relative, 2-norm)
+// where m >= 64 (64 x 576 6.8e-4, 512 x 2304 6.4e-4, 4096 x 4096 6.0e-4), up to 2e-3 from 16 rows and up to 3e-3 below, where few
+// singular values average less; six steps are a third more.  A bf16 update's rounding alone is 1.7e-3.  In a simulation bf16 operands were 4e-3 .. 2e-2 off, f16 without the pair 2e-3 .. 5e-3.
 //
 // Layout.  The workspace holds every matrix as blocks of 128 rows x 64 columns, 128 bytes a row, block after block: one
 // tensor map over the whole workspace serves all operands of all matrices, whatever their shapes.  A block is a K-major

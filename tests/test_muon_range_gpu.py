@@ -1,4 +1,6 @@
 """he_plan_muon on f32 gradients at the ends of f32's range, and on zero gradients with the smallest eps."""
+import ctypes
+
 import pytest
 
 import helium_b200 as hb
@@ -38,4 +40,19 @@ def test_a_zero_gradient_is_zero_for_any_eps(ctx, shape, eps):
     import torch
     (o,) = hb.Plan.muon(ctx, [shape], grad_dtype=ir.F32, momentum=None, eps=eps).launch([torch.zeros(shape, device="cuda")])
     assert torch.equal(o, torch.zeros_like(o))
+    ctx.poll()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("ratio", [1.0, 1e-2, 1e-3, 1e-4])
+def test_a_gradient_below_eps(ctx, shape, ratio):
+    """|d| / eps = ratio: X starts that much smaller, in f16 steps of 2^-24 whose root mean square is 1.7e-8.  The weakest singular
+    directions, ten times below the gradient's size, grow like the others: ten times 1.7e-8 / ratio, and a margin of two."""
+    g = _matrix(shape, 5)
+    eps = float(g.double().norm()) / ratio
+    (o,) = hb.Plan.muon(ctx, [shape], grad_dtype=ir.F32, momentum=None, eps=eps).launch([g])
+    eps = ctypes.c_float(eps).value
+    want, _ = _reference(g, None, None, False, 5, eps=eps)
+    tol = _tolerance(ir.BF16, 5, g, eps=eps) + 20 * 1.7e-8 * (1 + ratio) / ratio
+    _check(o, want, tol, f"{shape} {ratio}")
     ctx.poll()

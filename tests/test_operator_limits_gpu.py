@@ -187,3 +187,53 @@ def test_a_closed_plan_is_refused(ctx):
     plan.close()
     with pytest.raises(hb.HeliumError, match="null"):
         plan.launch([x, gamma, beta])
+
+
+@pytest.mark.parametrize("dt", [ir.BF16, ir.F32])
+@pytest.mark.parametrize("size", [(1, 4, 65536, 1), (2, 301, 65536, 2), (3, 5, 65535, 1), (1, 2, 65536, 32768), (1, 1, 65521, 1)])
+def test_the_most_channels(ctx, size, dt):
+    import torch
+    n, p, c, groups = size
+    x, gamma, beta, dy = _inputs(n, p, c, dt, 6)
+    plan = hb.Plan.group_norm(ctx, "fwd", n, p, c, groups, dtype=dt, activation="gelu")
+    y, mean, rstd = plan.launch([x, gamma, beta])
+    _check_forward(plan, x, gamma, beta, groups, "gelu", dt, y, mean, rstd)
+    dx, dgamma, dbeta = hb.Plan.group_norm(ctx, "bwd", n, p, c, groups, dtype=dt).launch([dy, x, gamma, beta, mean, rstd])
+    want, size_of = dy.double().sum((0, 1)), dy.double().abs().sum((0, 1))
+    assert bool(((dbeta.double() - want).abs() <= 64 * 2.0 ** -24 * size_of).all()) and not bool(torch.isnan(dx).any())
+
+
+@pytest.mark.parametrize("p,c,groups", [((1 << 31) - 1, 1, 1), ((1 << 31) - 3, 2, 2)])
+def test_the_most_positions(ctx, p, c, groups):
+    """Values -1, 0 and 1 (and 1 to 3 forward): sums of whole numbers.  Forward, the largest sum is 2^32: f32 adds partial sums beyond
+    2^24 with half steps of 2^-24 each, some twenty of them behind one another: 32 u."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.empty(1, p, c, dtype=torch.bfloat16, device="cuda").random_(1, 4, generator=gen)
+    sums = [0.0, 0.0]
+    for k in range(0, p, 1 << 28):
+        v = x[0, k:k + (1 << 28)].float()                # whole numbers below 2^24 a block of sum()'s own
+        sums[0] = sums[0] + v.sum(0, dtype=torch.float64)
+        sums[1] = sums[1] + (v * v).sum(0, dtype=torch.float64)
+    mean64 = sums[0] / p
+    rstd64 = 1 / (sums[1] / p - mean64 ** 2 + 1e-5).sqrt()
+    one, zero = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    y, mean, rstd = hb.Plan.group_norm(ctx, "fwd", 1, p, c, groups).launch([x, one, zero])
+    u = 2.0 ** -24
+    assert bool(((mean[0].double() / mean64 - 1).abs() <= 32 * u).all()) and bool(((rstd[0].double() / rstd64 - 1).abs() <= 128 * u).all())
+    for rows in (slice(0, 4096), slice(p // 2, p // 2 + 4096), slice(p - 4096, p)):
+        want = (x[0, rows].double() - mean64) * rstd64
+        assert bool(((y[0, rows].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()), rows
+    del y
+    dy = torch.empty_like(x).random_(-1, 2, generator=gen)
+    m, r = torch.full((1, groups), 2.0, device="cuda"), torch.ones(1, groups, device="cuda")
+    dx, dgamma, dbeta = hb.Plan.group_norm(ctx, "bwd", 1, p, c, groups).launch([dy, x, one, zero, m, r])
+    wb, wg = 0.0, 0.0
+    for k in range(0, p, 1 << 28):
+        d = dy[0, k:k + (1 << 28)].float()
+        wb = wb + d.sum(0, dtype=torch.float64)
+        wg = wg + (d * (x[0, k:k + (1 << 28)].float() - 2)).sum(0, dtype=torch.float64)
+    assert torch.equal(dbeta.double(), wb) and torch.equal(dgamma.double(), wg)
+    for rows in (slice(0, 4096), slice(p // 2, p // 2 + 4096), slice(p - 4096, p)):
+        want = dy[0, rows].double() - wb / p - (x[0, rows].double() - 2) * wg / p
+        assert bool(((dx[0, rows].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-6).all()), rows
